@@ -35,7 +35,8 @@ typedef enum {
   LUNA_ERR_OVERFLOW = -7          /* sizes exceed the 32-bit graph index range */
 } luna_status;
 
-typedef enum { LUNA_F32 = 0, LUNA_F64 = 1 } luna_dtype;
+/* The convolution, the harmonics and the distance buckets take the first two, the operators over rows all four. */
+typedef enum { LUNA_F32 = 0, LUNA_F64 = 1, LUNA_BF16 = 2, LUNA_F16 = 3 } luna_dtype;
 
 /* Human-readable description of the last failure on the calling thread ("" if none). */
 LUNA_API const char* luna_last_error(void);
@@ -248,6 +249,78 @@ LUNA_API int luna_sh_bwd(const luna_sh_desc* desc, const void* v, const void* g,
 /* With rx[n,3] the cotangent of dx: sx[n,3] = d<rx,dx>/dv, sg[n,C] = d<rx,dx>/dg = J rx; null outputs skipped. */
 LUNA_API int luna_sh_dbl_bwd(const luna_sh_desc* desc, const void* v, const void* g, const void* rx, void* sx, void* sg,
                     int64_t n, void* stream);
+
+/* --------------------------------------------------------------------------------------------------------------
+ * Layer norm over irreps: rows of `num_blocks` blocks of mul channels with `components` = 2l+1 elements each, one after
+ * the other.  Every block is normalised alone: scalars (`scalar` = 1, components 1) lose their mean, all are divided by
+ * sqrt(share * sum of squares + eps) with share = 1/(mul*components) (normalization 0, "component") or 1/mul (1, "norm"),
+ * then multiplied by one weight per channel, and scalars get one bias per channel.  weight[sum of mul] and bias[sum of mul
+ * of the scalar blocks] are consecutive in block order; null means ones and zeros.  At most 32 blocks of at most 16384
+ * elements (LUNA_ERR_UNSUPPORTED beyond).  Sums are held in float (double for LUNA_F64), without atomics: the same call gives the same bits.
+ *
+ * stats: what the forward leaves for the others, rows * num_blocks pairs (mean, scale) of float or double, in block-major
+ * order; the forward skips it if null. */
+typedef struct {
+  int32_t dtype, num_blocks;
+  int32_t mul[32], components[32], scalar[32];
+  int32_t normalization;
+  double eps;
+} luna_norm_desc;
+/* Scratch for a call that wants a weight or bias gradient; never zero.  Negative: a luna_status. */
+LUNA_API int64_t luna_layer_norm_scratch_bytes(const luna_norm_desc* desc, int64_t rows);
+LUNA_API int luna_layer_norm_fwd(const luna_norm_desc* desc, const void* x, const void* weight, const void* bias, void* y,
+                                 void* stats, int64_t rows, void* stream);
+/* With g the cotangent of y: gx[rows, dim], gw, gb; null outputs are skipped. */
+LUNA_API int luna_layer_norm_bwd(const luna_norm_desc* desc, const void* x, const void* weight, const void* stats, const void* g,
+                                 void* gx, void* gw, void* gb, void* scratch, int64_t scratch_bytes, int64_t rows, void* stream);
+/* With rx, rw, rb the cotangents of gx, gw, gb (null: zero): hx, hw, hg, the derivatives of <rx,gx>+<rw,gw>+<rb,gb>
+ * with respect to x, weight and g; null outputs are skipped. */
+LUNA_API int luna_layer_norm_dbl_bwd(const luna_norm_desc* desc, const void* x, const void* weight, const void* stats,
+                                     const void* g, const void* rx, const void* rw, const void* rb, void* hx, void* hw, void* hg,
+                                     void* scratch, int64_t scratch_bytes, int64_t rows, void* stream);
+
+/* --------------------------------------------------------------------------------------------------------------
+ * A learned bias by distance.  luna_distance_buckets: out[i] = number of boundaries b <= |v_i| (compared as squares in
+ * double precision; boundaries ascending and not negative), for v[n,3] of LUNA_F32 or LUNA_F64.
+ * luna_relative_bias_fwd: out[edges, heads] = table[buckets[e], heads]; an edge whose bucket is no row of the table gets
+ * zeros.  luna_relative_bias_bwd: gtable[num_buckets, heads] = sums of g over the edges of each bucket, without atomics,
+ * in an order that depends on the sizes alone. */
+LUNA_API int luna_distance_buckets(int dtype, const void* v, const void* boundaries, int64_t num_boundaries, int32_t* out,
+                                   int64_t n, void* stream);
+LUNA_API int luna_relative_bias_fwd(int dtype, const void* table, const int32_t* buckets, void* out, int64_t edges,
+                                    int64_t num_buckets, int64_t heads, void* stream);
+LUNA_API int64_t luna_relative_bias_scratch_bytes(int dtype, int64_t edges, int64_t num_buckets, int64_t heads);
+LUNA_API int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* buckets, void* gtable, void* scratch,
+                                    int64_t scratch_bytes, int64_t edges, int64_t num_buckets, int64_t heads, void* stream);
+
+/* --------------------------------------------------------------------------------------------------------------
+ * Softmax over the in-edges of every node, for logits[num_edges, heads] whose edges are sorted by destination.
+ * Row i is the edges rowptr[i] .. rowptr[i+1]-1.  Where a node's edges are cut into several rows (so that a long row does
+ * not hold one multiprocessor), first[node] is the node's first row, node[row] the row's node; else both are null.
+ *
+ * forward:  alpha = softmax(logits + table[buckets]) over the unmasked edges of each node (mask[e] = 0: left out, alpha 0);
+ *           a node without any, or with logits of -inf only, gets zeros.  table, buckets, mask may be null.
+ * backward: glogits = alpha (g - sum alpha g), and gtable its sums by bucket (null: not wanted).  Where alpha is zero the
+ *           gradient is zero, whatever stands in g there.
+ * second:   with r, rtable the cotangents of glogits, gtable (null: zero), the derivatives with respect to alpha and g;
+ *           null outputs are skipped. */
+typedef struct {
+  int64_t num_rows, num_edges, num_nodes;
+  const int32_t* rowptr;
+  const int64_t* first;
+  const int64_t* node;
+} luna_row_table;
+/* num_buckets: 0 for calls without a gradient of a table. */
+LUNA_API int64_t luna_graph_softmax_scratch_bytes(int dtype, const luna_row_table* rows, int64_t heads, int64_t num_buckets);
+LUNA_API int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, const void* logits, const void* table,
+                                    const int32_t* buckets, const uint8_t* mask, void* alpha, int64_t heads,
+                                    int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream);
+LUNA_API int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g,
+                                    const int32_t* buckets, void* glogits, void* gtable, int64_t heads, int64_t num_buckets,
+                                    void* scratch, int64_t scratch_bytes, void* stream);
+LUNA_API int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
+                                        const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
+                                        int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* --------------------------------------------------------------------------------------------------------------
  * Measurement aid, no counterpart in the reference: launches register-resident chains of fused multiply-adds

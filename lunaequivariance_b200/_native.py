@@ -29,7 +29,7 @@ LUNA_ERR_SCRATCH = -5
 LUNA_ERR_DEVICE_TIMEOUT = -6
 LUNA_ERR_OVERFLOW = -7
 
-LUNA_F32, LUNA_F64 = 0, 1
+LUNA_F32, LUNA_F64, LUNA_BF16, LUNA_F16 = 0, 1, 2, 3
 
 _EXCEPTIONS = {
     LUNA_ERR_INVALID_ARGUMENT: ValueError,
@@ -84,6 +84,19 @@ class ShDesc(ctypes.Structure):
     ]
 
 
+class NormDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("num_blocks", ctypes.c_int32), ("mul", ctypes.c_int32 * 32),
+        ("components", ctypes.c_int32 * 32), ("scalar", ctypes.c_int32 * 32), ("normalization", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+    ]
+
+
+class RowTable(ctypes.Structure):
+    _fields_ = [("num_rows", ctypes.c_int64), ("num_edges", ctypes.c_int64), ("num_nodes", ctypes.c_int64),
+                ("rowptr", ctypes.c_void_p), ("first", ctypes.c_void_p), ("node", ctypes.c_void_p)]
+
+
 # name -> (restype, argtypes); mirrors include/luna_b200.h
 _P = ctypes.c_void_p
 _SIGNATURES = {
@@ -122,6 +135,21 @@ _SIGNATURES = {
     "luna_sh_fwd": (ctypes.c_int, [ctypes.POINTER(ShDesc), _P, _P, ctypes.c_int64, _P]),
     "luna_sh_bwd": (ctypes.c_int, [ctypes.POINTER(ShDesc), _P, _P, _P, ctypes.c_int64, _P]),
     "luna_sh_dbl_bwd": (ctypes.c_int, [ctypes.POINTER(ShDesc), _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
+    "luna_layer_norm_scratch_bytes": (ctypes.c_int64, [ctypes.POINTER(NormDesc), ctypes.c_int64]),
+    "luna_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(NormDesc), *[_P] * 5, ctypes.c_int64, _P]),
+    "luna_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(NormDesc), *[_P] * 8, ctypes.c_int64, ctypes.c_int64, _P]),
+    "luna_layer_norm_dbl_bwd": (ctypes.c_int, [ctypes.POINTER(NormDesc), *[_P] * 11, ctypes.c_int64, ctypes.c_int64, _P]),
+    "luna_distance_buckets": (ctypes.c_int, [ctypes.c_int, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P]),
+    "luna_relative_bias_fwd": (ctypes.c_int, [ctypes.c_int, _P, _P, _P, *[ctypes.c_int64] * 3, _P]),
+    "luna_relative_bias_scratch_bytes": (ctypes.c_int64, [ctypes.c_int, *[ctypes.c_int64] * 3]),
+    "luna_relative_bias_bwd": (ctypes.c_int, [ctypes.c_int, *[_P] * 4, *[ctypes.c_int64] * 4, _P]),
+    "luna_graph_softmax_scratch_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.POINTER(RowTable), *[ctypes.c_int64] * 2]),
+    "luna_graph_softmax_fwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
+                                              ctypes.c_int64, _P]),
+    "luna_graph_softmax_bwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
+                                              ctypes.c_int64, _P]),
+    "luna_graph_softmax_dbl_bwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 7, *[ctypes.c_int64] * 2,
+                                                  _P, ctypes.c_int64, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -199,4 +227,4 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 __all__ = ["library", "binding", "check", "last_error", "pointer", "current_stream", "dtype_code", "UvuPath", "UvuDesc",
-           "Graph", "GraphOut", "GraphPieces", "ShDesc", "EXPORTED_SYMBOLS", "LIBRARY_PATH"]
+           "Graph", "GraphOut", "GraphPieces", "ShDesc", "NormDesc", "RowTable", "EXPORTED_SYMBOLS", "LIBRARY_PATH"]

@@ -1,0 +1,388 @@
+// Softmax over the in-edges of every node, head by head, with a learned bias by buckets added to the logits.
+//
+// Edges are sorted by destination, so a row is a contiguous piece of the [edges, heads] arrays.  With z = logit + table[bucket]
+// (masked edges: -inf), m = max z and l = sum exp(z - m) over the row: alpha = exp(z - m) / l, zeros where nothing is left.
+//   backward   with D = sum alpha g:   dz = alpha (g - D)
+//   second     the cotangent r of dz, R = sum alpha r:   d/dg = alpha (r - R),   d/dalpha = r (g - D) - g R
+// Where alpha is zero nothing flows, whatever stands in g or r there.
+//
+// Bound by HBM: a row's values are read once and held in registers between its sums and its outputs, as far as they fit; the rest of
+// a longer row is read again from cache.  `lanes` threads of a warp share a row, or a whole CTA where rows are long; of them
+// `across` (a power of two) lie side by side over an edge's heads.  Rows of more than a thousand edges come cut into pieces: one
+// launch makes the pieces' sums, one joins those of each node, and one makes the outputs.
+#pragma once
+
+#include "rows.cuh"
+
+namespace luna {
+namespace softmax {
+
+using rows::Acc;
+
+constexpr int kThreads = 256;
+
+struct Rows {
+  const int32_t* rowptr;
+  int64_t count;
+  const int64_t* first;  // of a node's pieces; null where rows are not cut
+  const int64_t* node;   // of a piece
+  int64_t nodes;
+};
+
+struct Shape {
+  int heads, across, lanes;  // lanes: threads per row; more than 32 means the whole CTA
+  int num_buckets;
+};
+
+enum Order { kForward, kBackward, kSecond };
+enum Phase { kWhole, kSums, kApply };
+
+template <typename T>
+struct Operands {
+  const T *logits, *table, *alpha, *g, *r, *rtable;
+  const int32_t* buckets;
+  const uint8_t* mask;
+  T *out, *out2;
+};
+
+template <typename A>
+struct Pair {
+  A a, b;
+};
+
+// Sums or maxima over the threads that hold the same heads of one row.
+template <typename A, int VEC>
+struct Together {
+  const Shape& S;
+  A* exchange;  // [2][warps][32][VEC]
+  int turn = 0;
+  __device__ Together(const Shape& S_, A* exchange_) : S(S_), exchange(exchange_) {}
+
+  template <typename F>
+  __device__ __forceinline__ void all(A (&v)[VEC], F&& join) {
+    const int within = S.lanes < 32 ? S.lanes : 32;
+    for (int off = within >> 1; off >= S.across; off >>= 1)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) v[c] = join(v[c], __shfl_xor_sync(0xffffffffu, v[c], off));
+    if (S.lanes <= 32) return;
+    // two buffers by turns, so that one barrier is enough
+    constexpr int kWarps = kThreads / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    A* at = exchange + turn * kWarps * 32 * VEC;
+    turn ^= 1;
+    if (lane < S.across)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) at[(warp * 32 + lane) * VEC + c] = v[c];
+    __syncthreads();
+    const int mine = lane & (S.across - 1);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) v[c] = at[mine * VEC + c];
+    for (int other = 1; other < kWarps; ++other)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) v[c] = join(v[c], at[(other * 32 + mine) * VEC + c]);
+  }
+  __device__ __forceinline__ void sum(A (&v)[VEC]) {
+    all(v, [](A p, A q) { return p + q; });
+  }
+  __device__ __forceinline__ void max(A (&v)[VEC]) {
+    all(v, [](A p, A q) { return fmax(p, q); });
+  }
+};
+
+__device__ __forceinline__ float exponential(float v) { return expf(v); }
+__device__ __forceinline__ double exponential(double v) { return exp(v); }
+
+template <typename A>
+__device__ __forceinline__ A lowest() {
+  return -static_cast<A>(INFINITY);
+}
+
+template <typename T, int VEC, int K, int ORDER, int PHASE>
+__global__ void __launch_bounds__(kThreads)
+rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __restrict__ stats) {
+  using A = Acc<T>;
+  __shared__ A exchange[2 * kThreads * VEC];
+  Together<A, VEC> together(S, exchange);
+  const int lane = threadIdx.x & (S.lanes - 1);
+  const int slot = lane / S.across, slots = S.lanes / S.across;
+  const int head = (blockIdx.y * S.across + (lane & (S.across - 1))) * VEC;
+  const bool here = head < S.heads;
+  const int teams = kThreads / S.lanes, team = threadIdx.x / S.lanes;
+  const int ahead = S.lanes < 32 ? team % (32 / S.lanes) : 0;  // teams of this warp before this one: they leave together
+
+  auto table_row = [&](const T* __restrict__ table, int64_t e, A (&v)[VEC]) {
+    const int b = o.buckets[e];
+    if (b >= 0 && b < S.num_buckets) {
+      rows::load<T, VEC>(table + static_cast<int64_t>(b) * S.heads + head, v);
+    } else {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) v[c] = A(0);
+    }
+  };
+  // What an edge brings: z (forward), alpha and g, and r.
+  auto fetch = [&](int64_t e, A (&u)[VEC], A (&g)[VEC], A (&r)[VEC]) {
+    if constexpr (ORDER == kForward) {
+      if (o.mask && !o.mask[e]) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) u[c] = lowest<A>();
+        return;
+      }
+      rows::load<T, VEC>(o.logits + e * S.heads + head, u);
+      if (o.table) {
+        A t[VEC];
+        table_row(o.table, e, t);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) u[c] += t[c];
+      }
+    } else {
+      rows::load<T, VEC>(o.alpha + e * S.heads + head, u);
+      rows::load<T, VEC>(o.g + e * S.heads + head, g);
+      if constexpr (ORDER == kSecond) {
+        if (o.r) {
+          rows::load<T, VEC>(o.r + e * S.heads + head, r);
+        } else {
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) r[c] = A(0);
+        }
+        if (o.rtable) {
+          A t[VEC];
+          table_row(o.rtable, e, t);
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) r[c] += t[c];
+        }
+      }
+    }
+  };
+  auto put = [&](int64_t e, const A (&u)[VEC], const A (&g)[VEC], const A (&r)[VEC], const A (&a)[VEC], const A (&b)[VEC]) {
+    A v[VEC], w[VEC];
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      if constexpr (ORDER == kForward) {
+        v[c] = u[c] * b[c];
+      } else if constexpr (ORDER == kBackward) {
+        v[c] = u[c] != A(0) ? u[c] * (g[c] - a[c]) : A(0);
+      } else {
+        v[c] = u[c] != A(0) ? u[c] * (r[c] - b[c]) : A(0);
+        w[c] = u[c] != A(0) ? r[c] * (g[c] - a[c]) - g[c] * b[c] : A(0);
+      }
+    }
+    if (o.out) rows::store<T, VEC>(o.out + e * S.heads + head, v);
+    if constexpr (ORDER == kSecond) {
+      if (o.out2) rows::store<T, VEC>(o.out2 + e * S.heads + head, w);
+    }
+  };
+
+  const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team; row - ahead < R.count; row += step) {
+    int64_t begin = 0, end = 0;
+    if (row < R.count && here) {
+      begin = R.rowptr[row];
+      end = R.rowptr[row + 1];
+    }
+    begin += slot;
+    A u[K][VEC], g[K][VEC], r[K][VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t e = begin + k * slots;
+      if (e < end) fetch(e, u[k], g[k], r[k]);
+    }
+    const int64_t rest = begin + static_cast<int64_t>(K) * slots;
+    A a[VEC], b[VEC];  // forward: the largest logit and the sum; else D and R
+    if constexpr (PHASE != kApply) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        a[c] = ORDER == kForward ? lowest<A>() : A(0);
+        b[c] = A(0);
+      }
+      auto take = [&](const A (&p)[VEC], const A (&q)[VEC], const A (&s)[VEC]) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          if constexpr (ORDER == kForward) {
+            a[c] = fmax(a[c], p[c]);
+          } else {
+            a[c] += p[c] != A(0) ? p[c] * q[c] : A(0);
+            if constexpr (ORDER == kSecond) b[c] += p[c] != A(0) ? p[c] * s[c] : A(0);
+          }
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (begin + k * slots < end) take(u[k], g[k], r[k]);
+      for (int64_t e = rest; e < end; e += slots) {
+        A p[VEC], q[VEC], s[VEC];
+        fetch(e, p, q, s);
+        take(p, q, s);
+      }
+      if constexpr (ORDER == kForward) {
+        together.max(a);
+        A shift[VEC];
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) shift[c] = a[c] == lowest<A>() ? A(0) : a[c];  // nothing left, or nothing but NaN
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (begin + k * slots < end)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+              const A w = exponential(u[k][c] - shift[c]);
+              if constexpr (PHASE == kWhole) u[k][c] = w;
+              b[c] += w;
+            }
+        for (int64_t e = rest; e < end; e += slots) {
+          A p[VEC], q[VEC], s[VEC];
+          fetch(e, p, q, s);
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) b[c] += exponential(p[c] - shift[c]);
+        }
+        together.sum(b);
+      } else {
+        together.sum(a);
+        if constexpr (ORDER == kSecond) together.sum(b);
+      }
+    } else {
+      if (row < R.count && here) {
+        const int64_t at = R.first[R.node[row]] * S.heads + head;
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          const Pair<A> known = stats[at + c];
+          a[c] = known.a;
+          b[c] = known.b;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) a[c] = b[c] = A(0);
+      }
+    }
+    if constexpr (PHASE == kSums) {
+      if (row < R.count && here && slot == 0)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) stats[row * S.heads + head + c] = Pair<A>{a[c], b[c]};
+    } else {
+      if constexpr (ORDER == kForward) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          a[c] = a[c] == lowest<A>() ? A(0) : a[c];
+          b[c] = b[c] == A(0) ? A(0) : A(1) / b[c];
+        }
+        if constexpr (PHASE == kApply) {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (begin + k * slots < end)
+#pragma unroll
+              for (int c = 0; c < VEC; ++c) u[k][c] = exponential(u[k][c] - a[c]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int64_t e = begin + k * slots;
+        if (e < end) put(e, u[k], g[k], r[k], a, b);
+      }
+      for (int64_t e = rest; e < end; e += slots) {
+        A p[VEC], q[VEC], s[VEC];
+        fetch(e, p, q, s);
+        if constexpr (ORDER == kForward) {
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) p[c] = exponential(p[c] - a[c]);
+        }
+        put(e, p, q, s, a, b);
+      }
+    }
+  }
+}
+
+// Joins the sums of the pieces of every node that has several, in its first piece's place: a warp per node.
+template <typename A, bool FORWARD>
+__global__ void __launch_bounds__(kThreads)
+join_kernel(const Rows R, int heads, Pair<A>* __restrict__ stats) {
+  const int lane = threadIdx.x & 31;
+  const int64_t node = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (node >= R.nodes) return;
+  const int64_t first = R.first[node], pieces = (node + 1 < R.nodes ? R.first[node + 1] : R.count) - first;
+  if (pieces < 2) return;
+  for (int h = 0; h < heads; ++h) {
+    A a = FORWARD ? lowest<A>() : A(0), b = A(0);
+    for (int64_t p = lane; p < pieces; p += 32) {
+      const Pair<A> piece = stats[(first + p) * heads + h];
+      if (FORWARD) {
+        a = fmax(a, piece.a);
+      } else {
+        a += piece.a;
+        b += piece.b;
+      }
+    }
+    for (int off = 16; off; off >>= 1) {
+      const A other = __shfl_xor_sync(0xffffffffu, a, off);
+      a = FORWARD ? fmax(a, other) : a + other;
+    }
+    if (FORWARD) {
+      const A shift = a == lowest<A>() ? A(0) : a;
+      for (int64_t p = lane; p < pieces; p += 32) {
+        const Pair<A> piece = stats[(first + p) * heads + h];
+        // a piece without a largest logit has nothing (a sum of zero) or nothing but NaN, in its sum too
+        b += piece.a == lowest<A>() ? piece.b : piece.b * exponential(piece.a - shift);
+      }
+    }
+    for (int off = 16; off; off >>= 1) b += __shfl_xor_sync(0xffffffffu, b, off);
+    __syncwarp();  // all have read the first piece
+    if (lane == 0) stats[first * heads + h] = Pair<A>{a, b};
+  }
+}
+
+template <typename T, int VEC, int K, int ORDER, int PHASE>
+int start(const Rows& R, const Shape& S, const Operands<T>& o, Pair<Acc<T>>* stats, cudaStream_t stream) {
+  const int64_t ctas = ceil_div(R.count, kThreads / S.lanes), most = static_cast<int64_t>(rows::processors()) * 256;
+  const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most), static_cast<unsigned>(ceil_div(S.heads, S.across * VEC)));
+  rows_kernel<T, VEC, K, ORDER, PHASE><<<grid, kThreads, 0, stream>>>(R, S, o, stats);
+  LUNA_LAUNCH_CHECK("softmax over in-edges");
+  return LUNA_OK;
+}
+
+template <typename T, int VEC, int ORDER>
+int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch, cudaStream_t stream) {
+  constexpr int K = VEC * sizeof(Acc<T>) >= 32 ? 2 : VEC * sizeof(Acc<T>) >= 16 ? 4 : 8;
+  Shape S{};
+  S.heads = static_cast<int>(heads);
+  S.num_buckets = static_cast<int>(num_buckets);
+  const int64_t packets = heads / VEC;
+  S.across = packets >= 32 ? 32 : rows::next_power_of_two(packets);
+  // As many threads as hold a row somewhat longer than the mean; a CTA where a warp would read most of a row twice.
+  const int64_t mean = ceil_div(edges, R.count);
+  const int64_t wanted = ceil_div(mean + mean / 4, K) * S.across;
+  S.lanes = wanted > 128 ? kThreads : wanted >= 32 ? 32 : rows::next_power_of_two(wanted);
+  auto* stats = static_cast<Pair<Acc<T>>*>(scratch);
+  if (!R.first) return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
+  if (const int status = start<T, VEC, K, ORDER, kSums>(R, S, o, stats, stream)) return status;
+  join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(ceil_div(R.nodes, kThreads / 32)), kThreads, 0, stream>>>(R, S.heads, stats);
+  LUNA_LAUNCH_CHECK("softmax over in-edges: pieces");
+  return start<T, VEC, K, ORDER, kApply>(R, S, o, stats, stream);
+}
+
+template <typename T, int ORDER>
+int with_packets(int vec, const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch,
+                 cudaStream_t stream) {
+  if constexpr (sizeof(T) <= 2) {
+    if (vec == 8) return launch<T, 8, ORDER>(R, edges, heads, num_buckets, o, scratch, stream);
+  }
+  if constexpr (sizeof(T) <= 4) {
+    if (vec == 4) return launch<T, 4, ORDER>(R, edges, heads, num_buckets, o, scratch, stream);
+  }
+  if (vec == 2) return launch<T, 2, ORDER>(R, edges, heads, num_buckets, o, scratch, stream);
+  return launch<T, 1, ORDER>(R, edges, heads, num_buckets, o, scratch, stream);
+}
+
+template <typename T>
+int run(Order order, int vec, const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch,
+        cudaStream_t stream) {
+  if (order == kForward) return with_packets<T, kForward>(vec, R, edges, heads, num_buckets, o, scratch, stream);
+  if (order == kBackward) return with_packets<T, kBackward>(vec, R, edges, heads, num_buckets, o, scratch, stream);
+  return with_packets<T, kSecond>(vec, R, edges, heads, num_buckets, o, scratch, stream);
+}
+
+#define LUNA_SOFTMAX_RUN(T) \
+  int run<T>(Order, int, const Rows&, int64_t, int64_t, int64_t, const Operands<T>&, void*, cudaStream_t)
+extern template LUNA_SOFTMAX_RUN(float);
+extern template LUNA_SOFTMAX_RUN(double);
+extern template LUNA_SOFTMAX_RUN(rows::bf16);
+extern template LUNA_SOFTMAX_RUN(rows::f16);
+
+}  // namespace softmax
+}  // namespace luna

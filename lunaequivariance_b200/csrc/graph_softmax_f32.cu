@@ -1,0 +1,4 @@
+#include "graph_softmax.cuh"
+namespace luna::softmax {
+template LUNA_SOFTMAX_RUN(float);
+}

@@ -46,6 +46,18 @@ struct Api {
   decltype(&luna_sh_fwd) sh_fwd = nullptr;
   decltype(&luna_sh_bwd) sh_bwd = nullptr;
   decltype(&luna_sh_dbl_bwd) sh_dbl_bwd = nullptr;
+  decltype(&luna_layer_norm_scratch_bytes) norm_scratch_bytes = nullptr;
+  decltype(&luna_layer_norm_fwd) norm_fwd = nullptr;
+  decltype(&luna_layer_norm_bwd) norm_bwd = nullptr;
+  decltype(&luna_layer_norm_dbl_bwd) norm_dbl_bwd = nullptr;
+  decltype(&luna_distance_buckets) distance_buckets = nullptr;
+  decltype(&luna_relative_bias_fwd) bias_fwd = nullptr;
+  decltype(&luna_relative_bias_scratch_bytes) bias_scratch_bytes = nullptr;
+  decltype(&luna_relative_bias_bwd) bias_bwd = nullptr;
+  decltype(&luna_graph_softmax_scratch_bytes) softmax_scratch_bytes = nullptr;
+  decltype(&luna_graph_softmax_fwd) softmax_fwd = nullptr;
+  decltype(&luna_graph_softmax_bwd) softmax_bwd = nullptr;
+  decltype(&luna_graph_softmax_dbl_bwd) softmax_dbl_bwd = nullptr;
 } api;
 
 template <typename F>
@@ -70,6 +82,18 @@ void load(const std::string& path) {
   resolve(library, "luna_sh_fwd", api.sh_fwd);
   resolve(library, "luna_sh_bwd", api.sh_bwd);
   resolve(library, "luna_sh_dbl_bwd", api.sh_dbl_bwd);
+  resolve(library, "luna_layer_norm_scratch_bytes", api.norm_scratch_bytes);
+  resolve(library, "luna_layer_norm_fwd", api.norm_fwd);
+  resolve(library, "luna_layer_norm_bwd", api.norm_bwd);
+  resolve(library, "luna_layer_norm_dbl_bwd", api.norm_dbl_bwd);
+  resolve(library, "luna_distance_buckets", api.distance_buckets);
+  resolve(library, "luna_relative_bias_fwd", api.bias_fwd);
+  resolve(library, "luna_relative_bias_scratch_bytes", api.bias_scratch_bytes);
+  resolve(library, "luna_relative_bias_bwd", api.bias_bwd);
+  resolve(library, "luna_graph_softmax_scratch_bytes", api.softmax_scratch_bytes);
+  resolve(library, "luna_graph_softmax_fwd", api.softmax_fwd);
+  resolve(library, "luna_graph_softmax_bwd", api.softmax_bwd);
+  resolve(library, "luna_graph_softmax_dbl_bwd", api.softmax_dbl_bwd);
 }
 
 // A failed status as the exception Python raises for it.
@@ -725,6 +749,473 @@ Tensor harmonics(const HarmonicsPtr& h, const Tensor& v) {
   return !h->constant && tracked({&v}) ? ShForward::apply(v, h) : sh_forward(*h, v);
 }
 
+// ---- operators over rows: what they share ------------------------------------------------------------------------------------
+using Maybe = std::optional<Tensor>;
+const Tensor& of(const Maybe& t) {
+  static const Tensor none;
+  return t ? *t : none;
+}
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+int row_dtype(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return LUNA_F32;
+    case at::kDouble: return LUNA_F64;
+    case at::kBFloat16: return LUNA_BF16;
+    case at::kHalf: return LUNA_F16;
+    default: break;
+  }
+  TORCH_CHECK_TYPE(false, what, " requires float32, float64, bfloat16 or float16, got ", t.scalar_type());
+  return -1;
+}
+// `t` is an operand beside `x`: of its type unless another is named, on its device, of this shape.
+void check_beside(const Tensor& x, const Tensor& t, const char* name, at::IntArrayRef shape, std::optional<at::ScalarType> type = {}) {
+  if (!t.defined()) return;
+  TORCH_CHECK_TYPE(t.scalar_type() == type.value_or(x.scalar_type()), name, " must be ", type.value_or(x.scalar_type()), ", got ",
+                   t.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
+  TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
+}
+Tensor scratch_of(int64_t bytes, const Tensor& like) {
+  if (bytes < 0) check(static_cast<int>(bytes));
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+int64_t bytes_of(const Tensor& t) { return t.defined() ? t.numel() : 0; }
+
+// ---- layer norm ----------------------------------------------------------------------------------------------------------------
+struct Norm : torch::CustomClassHolder {
+  luna_norm_desc desc{};  // the type comes with each call
+  int64_t dim = 0, weights = 0, biases = 0;
+  Norm(const std::vector<std::array<int64_t, 3>>& blocks, int64_t normalization, double eps) {
+    TORCH_CHECK_NOT_IMPLEMENTED(blocks.size() <= 32, "layer norm of more than 32 blocks");
+    desc.num_blocks = static_cast<int32_t>(blocks.size());
+    desc.normalization = static_cast<int32_t>(normalization);
+    desc.eps = eps;
+    for (size_t i = 0; i < blocks.size(); ++i) {
+      const auto& [mul, components, scalar] = blocks[i];
+      desc.mul[i] = static_cast<int32_t>(mul);
+      desc.components[i] = static_cast<int32_t>(components);
+      desc.scalar[i] = static_cast<int32_t>(scalar);
+      dim += mul * components;
+      weights += mul;
+      biases += scalar ? mul : 0;
+    }
+  }
+  luna_norm_desc as(const Tensor& x) const {
+    luna_norm_desc d = desc;
+    d.dtype = row_dtype(x, "layer norm");
+    return d;
+  }
+};
+using NormPtr = c10::intrusive_ptr<Norm>;
+
+Tensor norm_rows(const Tensor& t, const Norm& n) { return t.defined() ? t.reshape({-1, n.dim}).contiguous() : t; }
+
+luna_norm_desc check_norm(const Norm& n, const Tensor& x, const Tensor& weight, const Tensor& bias) {
+  refuse_tangents({&x, &weight, &bias});
+  TORCH_CHECK(x.is_cuda(), "CUDA is required for layer norm in this library");
+  const luna_norm_desc desc = n.as(x);
+  TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) == n.dim, "layer norm input must have shape (..., ", n.dim, "), got ", x.sizes());
+  check_beside(x, weight, "weight", {n.weights});
+  check_beside(x, bias, "bias", {n.biases});
+  return desc;
+}
+
+std::array<Tensor, 2> norm_forward(const Norm& n, const Tensor& x, const Tensor& weight, const Tensor& bias, bool keep_stats) {
+  const luna_norm_desc desc = check_norm(n, x, weight, bias);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = norm_rows(x, n), w = contiguous(weight), b = contiguous(bias);
+  Tensor y = at::empty(x.sizes(), rows.options()), stats;
+  if (keep_stats)
+    stats = at::empty({desc.num_blocks, rows.size(0), 2}, rows.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat));
+  check(api.norm_fwd(&desc, rows.data_ptr(), pointer(w), pointer(b), y.data_ptr(), pointer(stats), rows.size(0), stream_of(x)));
+  return {y, stats};
+}
+
+// The gradients of x, weight and bias named in `mask`.
+std::array<Tensor, 3> norm_backward(const Norm& n, const Tensor& x, const Tensor& weight, const Tensor& stats, const Tensor& g, int mask) {
+  std::array<Tensor, 3> out;
+  if (!mask) return out;
+  const luna_norm_desc desc = check_norm(n, x, weight, Tensor());
+  refuse_tangents({&g});
+  check_beside(x, g, "grad_out", x.sizes());
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = norm_rows(x, n), w = contiguous(weight), cotangents = norm_rows(g, n);
+  if (mask & 1) out[0] = at::empty(x.sizes(), rows.options());
+  if (mask & 2) out[1] = at::empty({n.weights}, rows.options());
+  if (mask & 4) out[2] = at::empty({n.biases}, rows.options());
+  const Tensor scratch = mask & 6 ? scratch_of(api.norm_scratch_bytes(&desc, rows.size(0)), x) : Tensor();
+  check(api.norm_bwd(&desc, rows.data_ptr(), pointer(w), stats.data_ptr(), cotangents.data_ptr(), pointer(out[0]), pointer(out[1]),
+                     n.biases ? pointer(out[2]) : nullptr, pointer(scratch), bytes_of(scratch), rows.size(0), stream_of(x)));
+  return out;
+}
+
+// The second derivatives of x, weight and g named in `mask`, for the cotangents of the three gradients.
+std::array<Tensor, 3> norm_double(const Norm& n, const Tensor& x, const Tensor& weight, const Tensor& stats, const Tensor& g,
+                                  const Tensor& rx, const Tensor& rw, const Tensor& rb, int mask) {
+  std::array<Tensor, 3> out;
+  if (!mask) return out;
+  const luna_norm_desc desc = check_norm(n, x, weight, Tensor());
+  refuse_tangents({&g, &rx, &rw, &rb});
+  check_beside(x, g, "grad_out", x.sizes());
+  check_beside(x, rx, "rx", x.sizes());
+  check_beside(x, rw, "rw", {n.weights});
+  check_beside(x, rb, "rb", {n.biases});
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = norm_rows(x, n), w = contiguous(weight), cotangents = norm_rows(g, n), tx = norm_rows(rx, n), tw = contiguous(rw),
+               tb = contiguous(rb);
+  if (mask & 1) out[0] = at::empty(x.sizes(), rows.options());
+  if (mask & 2) out[1] = at::empty({n.weights}, rows.options());
+  if (mask & 4) out[2] = at::empty(x.sizes(), rows.options());
+  const Tensor scratch = mask & 2 ? scratch_of(api.norm_scratch_bytes(&desc, rows.size(0)), x) : Tensor();
+  check(api.norm_dbl_bwd(&desc, rows.data_ptr(), pointer(w), stats.data_ptr(), cotangents.data_ptr(), pointer(tx), pointer(tw),
+                         n.biases ? pointer(tb) : nullptr, pointer(out[0]), pointer(out[1]), pointer(out[2]), pointer(scratch),
+                         bytes_of(scratch), rows.size(0), stream_of(x)));
+  return out;
+}
+
+// Which of these tensors' gradients the running task wants: an edge belongs to each tensor that is there.
+int wanted(AutogradContext* ctx, std::initializer_list<const Tensor*> tensors) {
+  int mask = 0, bit = 0, edge = 0;
+  for (const Tensor* t : tensors) {
+    if (t->defined() && ctx->needs_input_grad(edge++)) mask |= 1 << bit;
+    ++bit;
+  }
+  return mask;
+}
+
+struct NormDouble : Function<NormDouble> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight, const Tensor& g, const Tensor& stats,
+                               const Maybe& rx, const Maybe& rw, const Maybe& rb, int64_t mask, const NormPtr& n) {
+    ctx->set_materialize_grads(false);
+    return only(norm_double(*n, x, of(weight), stats, g, of(rx), of(rw), of(rb), static_cast<int>(mask)), static_cast<int>(mask));
+  }
+  static variable_list backward(AutogradContext*, const variable_list& grads) {
+    for (const Tensor& t : grads)
+      TORCH_CHECK_NOT_IMPLEMENTED(!t.defined(), "third-order derivatives of the layer norm are not provided");
+    return variable_list(9);
+  }
+};
+
+struct NormBackward : Function<NormBackward> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight, const Tensor& g, const Tensor& stats,
+                               int64_t mask, const NormPtr& n) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, of(weight), g, stats});
+    ctx->saved_data["mask"] = mask;
+    keep(ctx, "norm", n);
+    return only(norm_backward(*n, x, of(weight), stats, g, static_cast<int>(mask)), static_cast<int>(mask));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    const auto r = spread<3>(grads, static_cast<int>(ctx->saved_data["mask"].toInt()));
+    if (!r[0].defined() && !r[1].defined() && !r[2].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int mask = wanted(ctx, {&saved[0], &saved[1], &saved[2]});
+    if (!mask) return out;
+    const auto n = kept<Norm>(ctx, "norm");
+    const auto h = at::GradMode::is_enabled()
+                       ? spread<3>(NormDouble::apply(saved[0], maybe(saved[1]), saved[2], saved[3], maybe(r[0]), maybe(r[1]), maybe(r[2]),
+                                                     static_cast<int64_t>(mask), n), mask)
+                       : norm_double(*n, saved[0], saved[1], saved[3], saved[2], r[0], r[1], r[2], mask);
+    for (int s = 0; s < 3; ++s) out[s] = h[s];
+    return out;
+  }
+};
+
+struct NormForward : Function<NormForward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight, const Maybe& bias, const NormPtr& n) {
+    const auto found = norm_forward(*n, x, of(weight), of(bias), true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, of(weight), found[1]});
+    ctx->saved_data["bias"] = bias.has_value();
+    keep(ctx, "norm", n);
+    return found[0];
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const auto n = kept<Norm>(ctx, "norm");
+    int mask = wanted(ctx, {&saved[0], &saved[1]});
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(saved[1].defined() ? 2 : 1)) mask |= 4;
+    if (!mask) return out;
+    const auto d = at::GradMode::is_enabled()
+                       ? spread<3>(NormBackward::apply(saved[0], maybe(saved[1]), grads[0], saved[2], static_cast<int64_t>(mask), n), mask)
+                       : norm_backward(*n, saved[0], saved[1], saved[2], grads[0], mask);
+    for (int s = 0; s < 3; ++s) out[s] = d[s];
+    return out;
+  }
+};
+
+Tensor layer_norm(const NormPtr& n, const Tensor& x, const Maybe& weight, const Maybe& bias) {
+  pybind11::gil_scoped_release release;
+  return tracked({&x, &of(weight), &of(bias)}) ? NormForward::apply(x, weight, bias, n)
+                                               : norm_forward(*n, x, of(weight), of(bias), false)[0];
+}
+
+// ---- bias by buckets -------------------------------------------------------------------------------------------------------------
+Tensor distance_buckets(const Tensor& v, const Tensor& boundaries) {
+  pybind11::gil_scoped_release release;
+  TORCH_CHECK(v.is_cuda(), "CUDA is required for distance buckets in this library");
+  TORCH_CHECK_TYPE(v.scalar_type() == at::kFloat || v.scalar_type() == at::kDouble, "distance buckets require float32 or float64 vectors, got ",
+                   v.scalar_type());
+  TORCH_CHECK_VALUE(v.dim() > 0 && v.size(-1) == 3, "distance buckets require vectors of shape (...,3), got ", v.sizes());
+  TORCH_CHECK_VALUE(boundaries.dim() == 1, "boundaries must be one-dimensional, got ", boundaries.sizes());
+  check_beside(v, boundaries, "boundaries", boundaries.sizes());
+  const c10::cuda::CUDAGuard guard(v.device());
+  const Tensor flat = rows_of(v), borders = boundaries.contiguous();
+  Tensor out = at::empty(v.sizes().slice(0, v.dim() - 1), v.options().dtype(at::kInt));
+  check(api.distance_buckets(v.scalar_type() == at::kDouble ? LUNA_F64 : LUNA_F32, flat.data_ptr(), borders.data_ptr(), borders.numel(),
+                             out.data_ptr<int32_t>(), flat.size(0), stream_of(v)));
+  return out;
+}
+
+void check_buckets(const Tensor& beside, const Tensor& buckets) {
+  TORCH_CHECK(beside.is_cuda(), "CUDA is required for the relative bias in this library");
+  TORCH_CHECK_TYPE(buckets.scalar_type() == at::kInt, "buckets must be Int, got ", buckets.scalar_type());
+  TORCH_CHECK_VALUE(buckets.device() == beside.device(), "buckets must be on ", beside.device(), ", got ", buckets.device());
+}
+
+Tensor bias_forward(const Tensor& table, const Tensor& buckets) {
+  refuse_tangents({&table});
+  check_buckets(table, buckets);
+  const int dtype = row_dtype(table, "relative bias");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0, "the bias table must have shape (buckets, heads), got ",
+                    table.sizes());
+  const c10::cuda::CUDAGuard guard(table.device());
+  const Tensor t = table.contiguous(), b = buckets.contiguous();
+  auto shape = buckets.sizes().vec();
+  shape.push_back(table.size(1));
+  Tensor out = at::empty(shape, table.options());
+  check(api.bias_fwd(dtype, t.data_ptr(), b.data_ptr<int32_t>(), out.data_ptr(), b.numel(), t.size(0), t.size(1), stream_of(t)));
+  return out;
+}
+
+Tensor bias_backward(const Tensor& g, const Tensor& buckets, int64_t num_buckets) {
+  refuse_tangents({&g});
+  check_buckets(g, buckets);
+  const int dtype = row_dtype(g, "relative bias");
+  TORCH_CHECK_VALUE(g.dim() == buckets.dim() + 1 && g.sizes().slice(0, buckets.dim()) == buckets.sizes() && g.size(-1) > 0,
+                    "the gradient of a bias must have shape (*buckets, heads), got ", g.sizes());
+  const c10::cuda::CUDAGuard guard(g.device());
+  const Tensor e = g.contiguous(), b = buckets.contiguous();
+  Tensor out = at::empty({num_buckets, g.size(-1)}, g.options());
+  const Tensor scratch = scratch_of(api.bias_scratch_bytes(dtype, b.numel(), num_buckets, g.size(-1)), g);
+  check(api.bias_bwd(dtype, e.data_ptr(), b.data_ptr<int32_t>(), out.data_ptr(), pointer(scratch), bytes_of(scratch), b.numel(), num_buckets,
+                     g.size(-1), stream_of(g)));
+  return out;
+}
+
+// Linear, and each the other's derivative: every order is there.
+struct BiasBackward;
+struct BiasForward : Function<BiasForward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& buckets);
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads);
+};
+struct BiasBackward : Function<BiasBackward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& g, const Tensor& buckets, int64_t num_buckets);
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads);
+};
+Tensor BiasForward::forward(AutogradContext* ctx, const Tensor& table, const Tensor& buckets) {
+  ctx->set_materialize_grads(false);
+  ctx->save_for_backward({buckets});
+  ctx->saved_data["buckets"] = table.dim() ? table.size(0) : 0;
+  return bias_forward(table, buckets);
+}
+variable_list BiasForward::backward(AutogradContext* ctx, const variable_list& grads) {
+  if (!grads[0].defined()) return variable_list(2);
+  const Tensor buckets = ctx->get_saved_variables()[0];
+  const int64_t count = ctx->saved_data["buckets"].toInt();
+  return {tracked({&grads[0]}) ? BiasBackward::apply(grads[0], buckets, count) : bias_backward(grads[0], buckets, count), Tensor()};
+}
+Tensor BiasBackward::forward(AutogradContext* ctx, const Tensor& g, const Tensor& buckets, int64_t num_buckets) {
+  ctx->set_materialize_grads(false);
+  ctx->save_for_backward({buckets});
+  return bias_backward(g, buckets, num_buckets);
+}
+variable_list BiasBackward::backward(AutogradContext* ctx, const variable_list& grads) {
+  if (!grads[0].defined()) return variable_list(3);
+  const Tensor buckets = ctx->get_saved_variables()[0];
+  return {tracked({&grads[0]}) ? BiasForward::apply(grads[0], buckets) : bias_forward(grads[0], buckets), Tensor(), Tensor()};
+}
+
+Tensor relative_bias(const Tensor& table, const Tensor& buckets) {
+  pybind11::gil_scoped_release release;
+  return tracked({&table}) ? BiasForward::apply(table, buckets) : bias_forward(table, buckets);
+}
+
+// ---- softmax over in-edges ----------------------------------------------------------------------------------------------------------
+struct Rows : torch::CustomClassHolder {
+  std::array<Tensor, 3> tables;  // rowptr; of cut rows the first piece of each node and the node of each piece
+  luna_row_table native{};
+  Rows(const Tensor& rowptr, int64_t edges, const Maybe& first, const Maybe& node) : tables{rowptr, of(first), of(node)} {
+    native.num_rows = rowptr.numel() - 1;
+    native.num_edges = edges;
+    native.rowptr = rowptr.data_ptr<int32_t>();
+    native.num_nodes = native.num_rows;
+    if (!first) return;
+    native.num_nodes = first->numel();
+    native.first = first->data_ptr<int64_t>();
+    native.node = node->data_ptr<int64_t>();
+  }
+};
+using RowsPtr = c10::intrusive_ptr<Rows>;
+
+int check_softmax(const Rows& rows, const Tensor& x, const char* name) {
+  refuse_tangents({&x});
+  TORCH_CHECK(x.is_cuda(), "CUDA is required for the softmax over in-edges in this library");
+  const int dtype = row_dtype(x, "the softmax over in-edges");
+  TORCH_CHECK_VALUE((x.dim() == 1 || x.dim() == 2) && x.size(0) == rows.native.num_edges && (x.dim() == 1 || x.size(1) > 0), name,
+                    " must have shape (", rows.native.num_edges, ") or (", rows.native.num_edges, ", heads), got ", x.sizes());
+  TORCH_CHECK_VALUE(rows.tables[0].device() == x.device() || !rows.native.num_edges, "logits and graph must share one CUDA device");
+  return dtype;
+}
+int64_t heads_of(const Tensor& x) { return x.dim() == 2 ? x.size(1) : 1; }
+void check_table(const Tensor& x, const Tensor& table, const Tensor& buckets) {
+  if (table.defined())
+    TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) > 0, "the bias table must have shape (buckets, heads), got ", table.sizes());
+  check_beside(x, table, "table", {table.defined() ? table.size(0) : 0, heads_of(x)});
+  check_beside(x, buckets, "buckets", {x.size(0)}, at::kInt);
+}
+
+Tensor softmax_forward(const Rows& rows, const Tensor& logits, const Tensor& table, const Tensor& buckets, const Tensor& mask) {
+  const int dtype = check_softmax(rows, logits, "logits");
+  refuse_tangents({&table});
+  TORCH_CHECK_VALUE(table.defined() == buckets.defined(), "a bias table and the edges' buckets come together");
+  check_table(logits, table, buckets);
+  check_beside(logits, mask, "mask", {logits.size(0)}, at::kBool);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor z = logits.contiguous(), t = contiguous(table), b = contiguous(buckets), m = contiguous(mask);
+  Tensor alpha = at::empty(z.sizes(), z.options());
+  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(z), 0), z);
+  check(api.softmax_fwd(dtype, &rows.native, z.data_ptr(), pointer(t), static_cast<const int32_t*>(pointer(b)),
+                        static_cast<const uint8_t*>(pointer(m)), alpha.data_ptr(), heads_of(z), t.defined() ? t.size(0) : 0,
+                        pointer(scratch), bytes_of(scratch), stream_of(z)));
+  return alpha;
+}
+
+// The gradients of the logits and of the table, as far as `mask` names them.
+std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, const Tensor& g, const Tensor& buckets, int64_t num_buckets,
+                                       int mask) {
+  std::array<Tensor, 2> out;
+  if (!mask) return out;
+  const int dtype = check_softmax(rows, alpha, "alpha");
+  refuse_tangents({&g});
+  check_beside(alpha, g, "grad_out", alpha.sizes());
+  check_table(alpha, Tensor(), buckets);
+  const c10::cuda::CUDAGuard guard(alpha.device());
+  const Tensor a = alpha.contiguous(), e = g.contiguous(), b = contiguous(buckets);
+  out[0] = at::empty(a.sizes(), a.options());  // the table's gradient is made of it
+  if (mask & 2) out[1] = at::empty({num_buckets, heads_of(a)}, a.options());
+  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(a), mask & 2 ? num_buckets : 0), a);
+  check(api.softmax_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), static_cast<const int32_t*>(pointer(b)), out[0].data_ptr(),
+                        pointer(out[1]), heads_of(a), num_buckets, pointer(scratch), bytes_of(scratch), stream_of(a)));
+  if (!(mask & 1)) out[0] = Tensor();
+  return out;
+}
+
+// The derivatives with respect to alpha and g named in `mask`.
+std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, const Tensor& g, const Tensor& buckets, const Tensor& r,
+                                     const Tensor& rtable, int mask) {
+  std::array<Tensor, 2> out;
+  if (!mask) return out;
+  const int dtype = check_softmax(rows, alpha, "alpha");
+  refuse_tangents({&g, &r, &rtable});
+  check_beside(alpha, g, "grad_out", alpha.sizes());
+  check_beside(alpha, r, "r", alpha.sizes());
+  check_table(alpha, rtable, buckets);
+  const c10::cuda::CUDAGuard guard(alpha.device());
+  const Tensor a = alpha.contiguous(), e = g.contiguous(), b = contiguous(buckets), t = contiguous(r), tt = contiguous(rtable);
+  for (int s = 0; s < 2; ++s)
+    if (mask >> s & 1) out[s] = at::empty(a.sizes(), a.options());
+  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(a), 0), a);
+  check(api.softmax_dbl_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), pointer(t), pointer(tt), static_cast<const int32_t*>(pointer(b)),
+                            pointer(out[0]), pointer(out[1]), heads_of(a), tt.defined() ? tt.size(0) : 0, pointer(scratch), bytes_of(scratch),
+                            stream_of(a)));
+  return out;
+}
+
+struct SoftmaxDouble : Function<SoftmaxDouble> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
+                               const Maybe& rtable, int64_t mask, const RowsPtr& rows) {
+    ctx->set_materialize_grads(false);
+    return only(softmax_double(*rows, alpha, g, of(buckets), of(r), of(rtable), static_cast<int>(mask)), static_cast<int>(mask));
+  }
+  static variable_list backward(AutogradContext*, const variable_list& grads) {
+    for (const Tensor& t : grads)
+      TORCH_CHECK_NOT_IMPLEMENTED(!t.defined(), "third-order derivatives of the softmax over in-edges are not provided");
+    return variable_list(7);
+  }
+};
+
+struct SoftmaxBackward : Function<SoftmaxBackward> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
+                               int64_t mask, const RowsPtr& rows) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({alpha, g, of(buckets)});
+    ctx->saved_data["mask"] = mask;
+    keep(ctx, "rows", rows);
+    return only(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, static_cast<int>(mask)), static_cast<int>(mask));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    const auto r = spread<2>(grads, static_cast<int>(ctx->saved_data["mask"].toInt()));
+    if (!r[0].defined() && !r[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int mask = wanted(ctx, {&saved[0], &saved[1]});
+    if (!mask) return out;
+    const auto rows = kept<Rows>(ctx, "rows");
+    const auto h = at::GradMode::is_enabled()
+                       ? spread<2>(SoftmaxDouble::apply(saved[0], saved[1], maybe(saved[2]), maybe(r[0]), maybe(r[1]),
+                                                        static_cast<int64_t>(mask), rows), mask)
+                       : softmax_double(*rows, saved[0], saved[1], saved[2], r[0], r[1], mask);
+    for (int s = 0; s < 2; ++s) out[s] = h[s];
+    return out;
+  }
+};
+
+struct SoftmaxForward : Function<SoftmaxForward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask,
+                        const RowsPtr& rows) {
+    const Tensor alpha = softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({alpha, of(buckets)});  // alpha says all about the logits, the table and the mask
+    ctx->saved_data["buckets"] = table ? table->size(0) : 0;
+    keep(ctx, "rows", rows);
+    return alpha;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int64_t num_buckets = ctx->saved_data["buckets"].toInt();
+    int mask = ctx->needs_input_grad(0) ? 1 : 0;
+    if (num_buckets && ctx->needs_input_grad(1)) mask |= 2;
+    if (!mask) return out;
+    const auto rows = kept<Rows>(ctx, "rows");
+    const auto d = at::GradMode::is_enabled()
+                       ? spread<2>(SoftmaxBackward::apply(saved[0], grads[0], maybe(saved[1]), num_buckets, static_cast<int64_t>(mask), rows), mask)
+                       : softmax_backward(*rows, saved[0], grads[0], saved[1], num_buckets, mask);
+    for (int s = 0; s < 2; ++s) out[s] = d[s];
+    return out;
+  }
+};
+
+Tensor graph_softmax(const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
+  pybind11::gil_scoped_release release;
+  return tracked({&logits, &of(table)}) ? SoftmaxForward::apply(logits, table, buckets, mask, rows)
+                                        : softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+}
+
+// The launches alone, for the operators that a traced program names.
+template <size_t N>
+std::vector<Maybe> listed(const std::array<Tensor, N>& tensors) {
+  std::vector<Maybe> list;
+  for (const Tensor& t : tensors) list.push_back(maybe(t));
+  return list;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(luna_torch, m) {
@@ -736,4 +1227,31 @@ PYBIND11_MODULE(luna_torch, m) {
   m.def("graph_tables", torch::wrap_pybind_function(graph_tables));
   m.def("conv", torch::wrap_pybind_function(conv));
   m.def("harmonics", torch::wrap_pybind_function(harmonics));
+  py::class_<Norm, NormPtr>(m, "Norm").def(py::init<const std::vector<std::array<int64_t, 3>>&, int64_t, double>());
+  py::class_<Rows, RowsPtr>(m, "Rows").def(py::init<const Tensor&, int64_t, const Maybe&, const Maybe&>());
+  m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
+  m.def("distance_buckets", torch::wrap_pybind_function(distance_buckets));
+  m.def("relative_bias", torch::wrap_pybind_function(relative_bias));
+  m.def("graph_softmax", torch::wrap_pybind_function(graph_softmax));
+  m.def("layer_norm_forward", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Maybe& bias) {
+    return listed(norm_forward(*n, x, of(weight), of(bias), true));
+  });
+  m.def("layer_norm_backward", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g, int mask) {
+    return listed(norm_backward(*n, x, of(weight), stats, g, mask));
+  });
+  m.def("layer_norm_double", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g,
+                                const Maybe& rx, const Maybe& rw, const Maybe& rb, int mask) {
+    return listed(norm_double(*n, x, of(weight), stats, g, of(rx), of(rw), of(rb), mask));
+  });
+  m.def("relative_bias_forward", torch::wrap_pybind_function(bias_forward));
+  m.def("relative_bias_backward", torch::wrap_pybind_function(bias_backward));
+  m.def("graph_softmax_forward", [](const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
+    return softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+  });
+  m.def("graph_softmax_backward", [](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
+                                     int mask) { return listed(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, mask)); });
+  m.def("graph_softmax_double", [](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
+                                   const Maybe& rtable, int mask) {
+    return listed(softmax_double(*rows, alpha, g, of(buckets), of(r), of(rtable), mask));
+  });
 }

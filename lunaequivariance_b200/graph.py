@@ -136,6 +136,17 @@ class LunaTPGraph:
                 self.source_rows)
         return holder
 
+    def row_holder(self):
+        """The rows of in-edges for the C++ launch path, long ones cut into pieces (``split_rows``)."""
+        holder = self._tables.get("rows")
+        if holder is None:
+            split = self.split_rows()
+            cut = split is not None and split.destinations.virtual_rows > self.num_nodes
+            holder = self._tables["rows"] = _native.binding().Rows(
+                split.graph.dst_rowptr if cut else self.dst_rowptr, self.num_edges,
+                split.destinations.first if cut else None, split.destinations.rows if cut else None)
+        return holder
+
     def destination_range(self, begin: int, end: int) -> "tuple[LunaTPGraph, int, int]":
         """The graph of the edges whose destination lies in ``[begin, end)``, and that slice ``[e0, e1)`` of the edge
         list: destinations renumbered from zero, sources as they are.

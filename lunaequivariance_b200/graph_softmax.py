@@ -1,0 +1,123 @@
+"""``graph_softmax``: softmax over the in-edges of every node, with a learned bias by buckets added on the way.
+
+The logits of an edge are one number per attention head, in the edge order of a graph (sorted by destination).  The result
+with one head is the ``env`` of a convolution: attention over a node's neighbours is a convolution whose messages are
+scaled by it.  Forward, backward (logits and bias table) and second order, without atomics.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from .conv import is_compiling
+from .graph import LunaTPGraph
+
+
+def _mask(needs) -> int:
+    return sum(1 << bit for bit, need in enumerate(needs) if need)
+
+
+# ----------------------------------------------------------------------------------------------- custom ops
+# A traced program carries the row pointers alone: rows are not cut, however long.
+
+
+def _rows(rowptr, edges):
+    return _native.binding().Rows(rowptr, edges, None, None)
+
+
+@torch.library.custom_op("lunaeq::graph_softmax_forward", mutates_args=())
+def graph_softmax_forward_op(logits: torch.Tensor, table: torch.Tensor | None, buckets: torch.Tensor | None,
+                             mask: torch.Tensor | None, rowptr: torch.Tensor, edges: int) -> torch.Tensor:
+    return _native.binding().graph_softmax_forward(_rows(rowptr, edges), logits, table, buckets, mask)
+
+
+@graph_softmax_forward_op.register_fake
+def _(logits, table, buckets, mask, rowptr, edges):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("lunaeq::graph_softmax_backward", mutates_args=(),
+                         schema="(Tensor alpha, Tensor g, Tensor? buckets, SymInt num_buckets, Tensor rowptr, bool[] needs)"
+                                " -> (Tensor?, Tensor?)")
+def graph_softmax_backward_op(alpha, g, buckets, num_buckets, rowptr, needs):
+    return tuple(_native.binding().graph_softmax_backward(_rows(rowptr, alpha.shape[0]), alpha, g, buckets, num_buckets,
+                                                          _mask(needs)))
+
+
+@graph_softmax_backward_op.register_fake
+def _(alpha, g, buckets, num_buckets, rowptr, needs):
+    heads = alpha.shape[1] if alpha.ndim == 2 else 1
+    return (torch.empty_like(alpha, memory_format=torch.contiguous_format) if needs[0] else None,
+            alpha.new_empty((num_buckets, heads)) if needs[1] else None)
+
+
+@torch.library.custom_op("lunaeq::graph_softmax_double_backward", mutates_args=(),
+                         schema="(Tensor alpha, Tensor g, Tensor? buckets, Tensor? r, Tensor? rtable, Tensor rowptr,"
+                                " bool[] needs) -> (Tensor?, Tensor?)")
+def graph_softmax_double_backward_op(alpha, g, buckets, r, rtable, rowptr, needs):
+    return tuple(_native.binding().graph_softmax_double(_rows(rowptr, alpha.shape[0]), alpha, g, buckets, r, rtable,
+                                                        _mask(needs)))
+
+
+@graph_softmax_double_backward_op.register_fake
+def _(alpha, g, buckets, r, rtable, rowptr, needs):
+    return tuple(torch.empty_like(alpha, memory_format=torch.contiguous_format) if need else None for need in needs)
+
+
+def _forward_setup(ctx, inputs, output):
+    _, table, buckets, _, rowptr, _ = inputs
+    ctx.num_buckets = 0 if table is None else table.shape[0]
+    ctx.save_for_backward(output, buckets, rowptr)
+    ctx.set_materialize_grads(False)
+
+
+def _forward_backward(ctx, g):
+    if g is None:
+        return (None,) * 6
+    alpha, buckets, rowptr = ctx.saved_tensors
+    needs = [ctx.needs_input_grad[0], bool(ctx.num_buckets) and ctx.needs_input_grad[1]]
+    return (*graph_softmax_backward_op(alpha, g, buckets, ctx.num_buckets, rowptr, needs), None, None, None, None)
+
+
+def _backward_setup(ctx, inputs, output):
+    alpha, g, buckets, _, rowptr, _ = inputs
+    ctx.save_for_backward(alpha, g, buckets, rowptr)
+    ctx.set_materialize_grads(False)
+
+
+def _backward_backward(ctx, r, rtable):
+    if r is None and rtable is None:
+        return (None,) * 6
+    alpha, g, buckets, rowptr = ctx.saved_tensors
+    return (*graph_softmax_double_backward_op(alpha, g, buckets, r, rtable, rowptr, list(ctx.needs_input_grad[:2])),
+            None, None, None, None)
+
+
+graph_softmax_forward_op.register_autograd(_forward_backward, setup_context=_forward_setup)
+graph_softmax_backward_op.register_autograd(_backward_backward, setup_context=_backward_setup)
+
+
+def graph_softmax(logits, graph, *, mask=None, table=None, buckets=None):
+    """Softmax of ``logits[edges]`` or ``logits[edges, heads]`` over the in-edges of every node of ``graph``.
+
+    ``table[buckets, heads]`` (of the type of the logits) and ``buckets[edges]`` (int32, as from ``distance_buckets``)
+    add a learned bias to the logits; a bucket that is no row of the table adds nothing.  ``mask[edges]`` (bool) keeps the
+    edges that are ``True``; what stands in the others' logits does not matter, and their result is zero.  A node whose
+    edges are all masked, or have logits of minus infinity only, gets zeros.
+    """
+    if not isinstance(graph, LunaTPGraph):
+        raise TypeError("graph must come from make_graph")
+    if (table is None) != (buckets is None):
+        raise TypeError("a bias table and the edges' buckets come together")
+    if is_compiling():
+        return torch.ops.lunaeq.graph_softmax_forward.default(logits, table, buckets, mask, graph.dst_rowptr,
+                                                              graph.num_edges)
+    if not logits.is_cuda:
+        raise RuntimeError("CUDA is required for the softmax over in-edges in this library")
+    if graph.src.device != logits.device and graph.num_edges:
+        raise ValueError("logits and graph must share one CUDA device")
+    return _native.binding().graph_softmax(graph.row_holder(), logits, table, buckets, mask)
+
+
+__all__ = ["graph_softmax"]

@@ -1,6 +1,6 @@
-"""``torch.nn.Module`` shells: ``TensorProductConv`` and ``SphericalHarmonics``.
+"""``torch.nn.Module`` shells: ``TensorProductConv``, ``TensorProduct``, ``SphericalHarmonics``, ``LayerNorm`` and ``RelativeBias``.
 
-Constructor arguments, attributes and dtype migration follow the reference's
+Of the first three, constructor arguments, attributes and dtype migration follow the reference's
 ``src/modules/tensorproduct.py:119-206`` and ``src/modules/spherical_harmonics.py:13-129``.
 """
 
@@ -13,7 +13,9 @@ import torch
 from .conv import create_uvu_conv_operator
 from .functional import require_uvu, resolve_source, tensor_product, tensor_product_conv
 from .graph import make_graph
+from .layer_norm import LayerNormConfig, layer_norm
 from .paths import TensorProductConfig
+from .relative_bias import distance_buckets, relative_bias
 from .tensor_product import LunaTPUVU
 from .spherical_harmonics import UNSET, SphericalHarmonicsConfig, spherical_harmonics
 
@@ -211,4 +213,74 @@ class SphericalHarmonics(torch.nn.Module):
 
 LunaEqSphericalHarmonics = SphericalHarmonics
 
-__all__ = ["TensorProductConv", "TensorProduct", "SphericalHarmonics", "LunaEqSphericalHarmonics"]
+
+class LayerNorm(torch.nn.Module):
+    """Layer norm over irreps (or over a number of scalars): see ``layer_norm``.
+
+    ``affine`` gives every channel a weight, and ``bias`` every ``0e`` channel a bias besides.
+    """
+
+    def __init__(self, irreps, eps=1e-5, affine=True, bias=True, normalization="component", *, device=None, dtype=None):
+        super().__init__()
+        self._config = LayerNormConfig(irreps, eps, normalization)
+        options = dict(device=device, dtype=dtype)
+        self.weight = torch.nn.Parameter(torch.ones(self._config.weight_numel, **options)) if affine else None
+        self.bias = (torch.nn.Parameter(torch.zeros(self._config.bias_numel, **options))
+                     if affine and bias and self._config.bias_numel else None)
+
+    irreps = property(lambda self: self._config.irreps)
+    eps = property(lambda self: self._config.eps)
+    normalization = property(lambda self: self._config.normalization)
+
+    def forward(self, x):
+        return layer_norm(x, weight=self.weight, bias=self.bias, config=self._config)
+
+    def extra_repr(self):
+        return f"{self.irreps}, eps={self.eps}, normalization={self.normalization}"
+
+
+class RelativeBias(torch.nn.Module):
+    """A learned row of ``heads`` numbers for every bucket of edge lengths between ``boundaries``.
+
+    ``boundaries`` are ascending numbers, none negative; ``k`` of them make ``k + 1`` buckets.  Calling the module gives
+    the bias of every edge vector; ``buckets`` gives the buckets alone, for ``graph_softmax(..., table=module.weight,
+    buckets=module.buckets(vec))``, which adds the bias without writing it to memory.
+    """
+
+    def __init__(self, boundaries, heads, *, device=None, dtype=None):
+        super().__init__()
+        self._boundaries = tuple(float(b) for b in boundaries)
+        if any(not 0.0 <= b < float("inf") for b in self._boundaries):
+            raise ValueError("boundaries must be finite and not negative")
+        if any(b < a for a, b in zip(self._boundaries, self._boundaries[1:])):
+            raise ValueError("boundaries must be in ascending order")
+        if heads < 1:
+            raise ValueError("RelativeBias needs a positive number of heads")
+        self.weight = torch.nn.Parameter(torch.zeros(len(self._boundaries) + 1, heads, device=device, dtype=dtype))
+        self._borders = {}
+
+    boundaries = property(lambda self: self._boundaries)
+
+    def _apply(self, fn, recurse=True):
+        result = super()._apply(fn, recurse=recurse)
+        self._borders = {}
+        return result
+
+    def buckets(self, vec):
+        """The bucket of every vector ``vec[..., 3]``, whatever the type of the weights."""
+        key = (vec.device, vec.dtype)
+        borders = self._borders.get(key)
+        if borders is None:
+            borders = self._borders[key] = torch.tensor(self._boundaries, device=vec.device, dtype=vec.dtype)
+        return distance_buckets(vec, borders)
+
+    def forward(self, vec):
+        return relative_bias(self.weight, self.buckets(vec))
+
+    def __getstate__(self):
+        return dict(super().__getstate__() if hasattr(super(), "__getstate__") else self.__dict__, _borders={})
+
+    def extra_repr(self):
+        return f"buckets={len(self._boundaries) + 1}, heads={self.weight.shape[1]}"
+
+__all__ = ["TensorProductConv", "TensorProduct", "SphericalHarmonics", "LunaEqSphericalHarmonics", "LayerNorm", "RelativeBias"]
