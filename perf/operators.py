@@ -175,7 +175,8 @@ def prepare(case, seed):
         if own:
             import lunaequivariance_b200 as luna
 
-            src = torch.randint(case["nodes"], (case["edges"],), generator=generator, device="cuda")
+            others = torch.Generator(device="cuda").manual_seed(seed + 1)  # the inputs do not depend on the sources
+            src = torch.randint(case["nodes"], (case["edges"],), generator=others, device="cuda")
             state["graph"] = luna.make_graph(src, state["dst"], case["nodes"])
     if case["order"] != "forward":
         state["g"] = normal(*shape)
