@@ -29,10 +29,12 @@ int describe(const luna_norm_desc* desc, int64_t rows, Params* P) {
     Block& B = P->block[i];
     B.offset = P->dim;
     B.length = mul * components;
+    B.channels = mul;
     B.components = components;
     B.scalar = desc->scalar[i] != 0;
     B.weight_offset = weights;
     B.bias_offset = biases;
+    B.inverse = static_cast<unsigned>(((1ull << 32) + components - 1) / components);
     B.share = 1.0 / (desc->normalization == 0 ? B.length : mul);
     P->dim += B.length;
     weights += mul;
@@ -46,13 +48,13 @@ int checked(const luna_norm_desc* desc, const void* p, const char* name, bool re
   return aligned_to(p, rows::size_of(desc->dtype)) ? LUNA_OK : fail(LUNA_ERR_MISALIGNED, "%s is not aligned to its element size", name);
 }
 
-int dispatch(Order order, const luna_norm_desc* desc, const Params& P, const Operands& o, void* stream) {
+int dispatch(Order order, const luna_norm_desc* desc, const Params& P, const Call& o, void* stream) {
   int status = LUNA_OK;
   rows::with_type(desc->dtype, [&](auto zero) { status = run<decltype(zero)>(order, P, o, static_cast<cudaStream_t>(stream)); });
   return status;
 }
 
-int check_scratch(const luna_norm_desc* desc, const Params& P, const Operands& o) {
+int check_scratch(const luna_norm_desc* desc, const Params& P, const Call& o) {
   if (!o.gw && !o.gb) return LUNA_OK;
   const int64_t needed = scratch_elements(P) * rows::acc_size_of(desc->dtype);
   if (!o.scratch || o.scratch_bytes < needed)
@@ -89,7 +91,7 @@ extern "C" int luna_layer_norm_fwd(const luna_norm_desc* desc, const void* x, co
   LUNA_TRY(checked(desc, weight, "weight", false));
   LUNA_TRY(checked(desc, bias, "bias", false));
   if (rows == 0) return LUNA_OK;
-  Operands o{};
+  Call o{};
   o.x = x, o.weight = weight, o.bias = bias, o.y = y, o.stats_out = stats;
   return dispatch(kForward, desc, P, o, stream);
 }
@@ -108,7 +110,7 @@ extern "C" int luna_layer_norm_bwd(const luna_norm_desc* desc, const void* x, co
   LUNA_TRY(checked(desc, gb, "gb", false));
   if (rows > 0 && !stats) return luna::fail(LUNA_ERR_INVALID_ARGUMENT, "stats is null");
   if (!gw && !gb && (!gx || rows == 0)) return LUNA_OK;
-  Operands o{};
+  Call o{};
   o.x = x, o.weight = weight, o.stats_in = stats, o.g = g, o.gx = gx, o.gw = gw, o.gb = gb, o.scratch = scratch,
   o.scratch_bytes = scratch_bytes;
   LUNA_TRY(check_scratch(desc, P, o));
@@ -133,7 +135,7 @@ extern "C" int luna_layer_norm_dbl_bwd(const luna_norm_desc* desc, const void* x
   LUNA_TRY(checked(desc, hg, "hg", false));
   if (rows > 0 && !stats) return luna::fail(LUNA_ERR_INVALID_ARGUMENT, "stats is null");
   if (!hw && ((!hx && !hg) || rows == 0)) return LUNA_OK;
-  Operands o{};
+  Call o{};
   o.x = x, o.weight = weight, o.stats_in = stats, o.g = g, o.rx = rx, o.rw = rw, o.rb = rb, o.hx = hx, o.gw = hw, o.hg = hg,
   o.scratch = scratch, o.scratch_bytes = scratch_bytes;
   LUNA_TRY(check_scratch(desc, P, o));

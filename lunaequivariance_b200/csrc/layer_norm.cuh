@@ -13,9 +13,15 @@
 // CTA) share a row, each with up to K packets of VEC elements, always the same columns, so that it keeps their weights and
 // the sums of the weights' gradients in registers from row to row.  Those sums meet once per CTA and once more in a second
 // launch, in an order that only the sizes decide: no atomics, the same bits every time.
+//
+// Rows arrive in shared memory by asynchronous copies, one round ahead of their use, so that the memory is busy while sums
+// are made.  Where rows are aligned, each thread copies what it will read itself and waits for nobody.  Rows that begin
+// anywhere in 16 bytes are moved a CTA's round of rows at a time, one contiguous chunk in aligned pieces, and read and written
+// number by number in shared memory (600,000 rows of 50 floats, forward: 77 us when global memory was read so).
+// Rows wider than a CTA of 256 holds, and unaligned blocks between others, are read when they are wanted.
 #pragma once
 
-#include <atomic>
+#include <type_traits>
 
 #include "rows.cuh"
 
@@ -27,10 +33,13 @@ using rows::Pack;
 
 constexpr int kMaxBlocks = 32;
 constexpr int kMaxLength = 16384;  // elements of a block
+constexpr int kThreads = 256, kWideThreads = 1024;
 
 struct Block {
-  int offset, length, components, scalar, weight_offset, bias_offset;
+  int offset, length, channels, components, scalar, weight_offset, bias_offset;
+  unsigned inverse;      // 2^32 / components, rounded up: i / components is the upper half of i * inverse for i <= kMaxLength
   int lanes;             // threads that share a row
+  int chunk;             // bytes of shared memory for a CTA's round of rows
   int first_cta, ctas;
   int64_t partial;       // first element of its CTAs' sums in the scratch buffer
   double share;
@@ -43,105 +52,253 @@ struct Params {
   Block block[kMaxBlocks];
 };
 
-__device__ __forceinline__ const Block& block_of(const Params& P) {
+__device__ __forceinline__ int block_index_of(const Params& P) {
   int i = 0;
   while (i + 1 < P.blocks && static_cast<int>(blockIdx.x) >= P.block[i + 1].first_cta) ++i;
-  return P.block[i];
+  return i;
 }
-
-// The threads that share a row, and their sums.
-template <typename A>
-struct Team {
-  int lanes, lane, index, teams;  // lane within the team, team within the CTA
-  A* exchange;                    // [2][warps of the CTA][kMaxSums]
-  int turn = 0;
-  static constexpr int kMaxSums = 8;
-
-  __device__ Team(int lanes_, A* exchange_) : lanes(lanes_), exchange(exchange_) {
-    lane = threadIdx.x & (lanes - 1);
-    index = threadIdx.x / lanes;
-    teams = blockDim.x / lanes;
-  }
-  // The first of the team's warp's rows decides when a warp leaves its loop: lanes of a warp stay together.
-  __device__ __forceinline__ int teams_before_warp() const { return lanes < 32 ? index - index % (32 / lanes) : index; }
-
-  template <int V>
-  __device__ __forceinline__ void sum(A (&v)[V]) {
-    for (int off = (lanes < 32 ? lanes : 32) >> 1; off; off >>= 1)
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
-    if (lanes <= 32) return;
-    // Two buffers by turns: who writes the first one again has passed the barrier after which nobody reads it.
-    const int warps = lanes >> 5, warp = threadIdx.x >> 5;
-    A* at = exchange + turn * (blockDim.x >> 5) * kMaxSums;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int i = 0; i < V; ++i) at[warp * kMaxSums + i] = v[i];
-    asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(lanes) : "memory");
-    const A* from = at + index * warps * kMaxSums;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = from[i];
-    for (int other = 1; other < warps; ++other)
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += from[other * kMaxSums + i];
-  }
-};
-
-// One thread's columns of a block: which they are, and their parameters.
-template <typename T, int VEC, int K>
-struct Columns {
-  using A = Acc<T>;
-  int first, step, length;
-  __device__ Columns(const Block& B, int lane) : first(lane * VEC), step(B.lanes * VEC), length(B.length) {}
-  __device__ __forceinline__ int at(int k) const { return first + k * step; }
-  __device__ __forceinline__ bool in(int k) const { return at(k) < length; }
-
-  __device__ __forceinline__ void parameters(const T* __restrict__ p, int offset, int components, A otherwise, A (&to)[K][VEC]) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) to[k][c] = p && in(k) ? rows::widen(p[offset + (at(k) + c) / components]) : otherwise;
-  }
-  __device__ __forceinline__ void load(const T* __restrict__ row, bool active, A (&to)[K][VEC]) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (active && in(k)) {
-        rows::load<T, VEC>(row + at(k), to[k]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) to[k][c] = A(0);
-      }
-    }
-  }
-};
 
 template <typename A>
 struct Moments {
   A mean, scale;
 };
 
-template <typename T, int VEC, int K, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-forward_kernel(const __grid_constant__ Params P, const T* __restrict__ x, const T* __restrict__ weight,
-               const T* __restrict__ bias, T* __restrict__ y, Moments<Acc<T>>* __restrict__ stats) {
+__device__ __forceinline__ void copy_16_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+constexpr int kMaxSums = 8;
+
+enum Mode { kPackets, kChunks, kDirect };
+constexpr int kStages = 2;  // rounds of rows on their way
+
+// A thread's place: which columns of the CTA's block it has, and of which rows.  LANES: threads of a warp that share a row;
+// where they are all of a warp, several warps may share it.  IN arrays are read, and chunks keep room for OUT.
+template <typename T, int VEC, int K, int LANES, int MODE, int IN, int OUT>
+struct Place {
   using A = Acc<T>;
-  __shared__ A exchange[2 * (THREADS / 32) * Team<A>::kMaxSums];
-  const Block& B = block_of(P);
-  Team<A> team(B.lanes, exchange);
-  const Columns<T, VEC, K> columns(B, team.lane);
+  static constexpr int kStep = LANES * VEC;   // from one of a thread's packets to the next
+  static constexpr int kPiece = kStep * K;    // columns of a warp
+  const Block& B;
+  int lane, warps, warp, team, teams;         // in the row's part of this warp; warps per row; of the row; row of the CTA
+  int begin, left;                            // first column of the warp's piece; columns from the thread's first one on
+  A* exchange;
+  unsigned char* shared;
+  int turn = 0, stage = 0;
+
+  __device__ __forceinline__ Place(const Block& B_, unsigned char* shared_, A* exchange_) : B(B_), exchange(exchange_), shared(shared_) {
+    const int in_cta = threadIdx.x >> 5;
+    lane = threadIdx.x & (LANES - 1);
+    warps = LANES == 32 ? B.lanes >> 5 : 1;
+    warp = LANES == 32 ? in_cta & (warps - 1) : 0;
+    team = LANES == 32 ? in_cta / warps : threadIdx.x / LANES;
+    teams = LANES == 32 ? (blockDim.x >> 5) / warps : blockDim.x / LANES;
+    begin = warp * kPiece;
+    left = B.length - begin - lane * VEC;
+  }
+  // Teams before this one whose loop this team shares: those of a warp, or of the CTA where it moves rows together.
+  __device__ __forceinline__ int ahead() const { return MODE == kChunks ? team : LANES == 32 ? 0 : (threadIdx.x & 31) / LANES; }
+  __device__ __forceinline__ bool in(int k) const { return k * kStep < left; }
+  __device__ __forceinline__ int column(int k) const { return begin + lane * VEC + k * kStep; }
+  __device__ __forceinline__ int channel(int i) const { return B.components == 1 ? i : static_cast<int>(__umulhi(i, B.inverse)); }
+  // Packets: a thread's own, those of a warp's threads side by side.  Chunks: one array's after the other's.
+  __device__ __forceinline__ unsigned char* packet(int array, int k) const { return shared + ((array * K + k) * blockDim.x + threadIdx.x) * 16; }
+  __device__ __forceinline__ unsigned char* chunk(int array) const { return shared + array * B.chunk; }
+  static __device__ __forceinline__ int shift_of(const T* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15); }
+
+  __device__ __forceinline__ void parameters(const T* __restrict__ p, int offset, A otherwise, A (&to)[K][VEC]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) to[k][c] = p && in(k) ? rows::widen(p[offset + channel(column(k) + c)]) : otherwise;
+  }
+
+  // Starts the copies of a round of rows, of which `row` is this team's, from arrays of P.rows rows.
+  __device__ __forceinline__ void request(const Params& P, const T* const (&arrays)[IN], int64_t row) {
+    if (MODE == kDirect) return;
+#pragma unroll
+    for (int a = 0; a < IN; ++a) {
+      if (!arrays[a]) continue;
+      if (MODE == kPackets) {
+        const T* from = arrays[a] + row * P.dim + B.offset + column(0);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (row < P.rows && in(k)) copy_16_async(packet(stage * IN + a, k), from + k * kStep);
+      } else {
+        const int64_t first = row - team, rest = P.rows - first;
+        if (rest <= 0) continue;
+        const int64_t numbers = (rest < teams ? rest : teams) * B.length;
+        const T* from = arrays[a] + first * B.length;
+        const int shift = shift_of(from), pieces = (shift + static_cast<int>(numbers * sizeof(T)) + 15) >> 4;
+        const unsigned char* base = reinterpret_cast<const unsigned char*>(from) - shift;
+        unsigned char* to = chunk(stage * IN + a);
+        for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+          // the first piece may begin before the array, and the last one end after it; another round is more than 16 bytes
+          if ((i > 0 || first > 0 || shift == 0) && (i + 1 < pieces || rest >= 2 * teams)) {
+            copy_16_async(to + i * 16, base + i * 16);
+          } else {
+            for (int j = i * 16; j < i * 16 + 16; j += static_cast<int>(sizeof(T)))
+              if (j >= shift && j < shift + static_cast<int>(numbers * sizeof(T)))
+                *reinterpret_cast<T*>(to + j) = *reinterpret_cast<const T*>(base + j);
+          }
+        }
+      }
+    }
+    commit_copies();
+    stage ^= 1;
+  }
+  // The oldest round of rows has come.
+  __device__ __forceinline__ void wait() {
+    if (MODE == kDirect) return;
+    wait_copies<kStages - 1>();
+    if (MODE == kChunks) __syncthreads();
+  }
+  // The thread's numbers of the oldest round; zeros where it has none.
+  __device__ __forceinline__ void take(const Params& P, int a, const T* array, int64_t row, A (&to)[K][VEC]) const {
+    const bool active = row < P.rows && array;
+    const T* from = array + row * P.dim + B.offset + column(0);
+    if (MODE == kChunks)
+      from = reinterpret_cast<const T*>(chunk(stage * IN + a) + shift_of(array + (row - team) * B.length)) + team * B.length + column(0);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (active && in(k)) {
+        rows::load<T, VEC>(MODE == kPackets ? reinterpret_cast<const T*>(packet(stage * IN + a, k)) : from + k * kStep, to[k]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) to[k][c] = A(0);
+      }
+    }
+  }
+  // Writes the thread's numbers of a row of output `a`; a chunk still has to be sent.
+  __device__ __forceinline__ void put(const Params& P, int a, T* array, int64_t row, const A (&from)[K][VEC]) const {
+    if (!array || row >= P.rows) return;
+    T* to = array + row * P.dim + B.offset + column(0);
+    if (MODE == kChunks)
+      to = reinterpret_cast<T*>(chunk(kStages * IN + a) + shift_of(array + (row - team) * B.length)) + team * B.length + column(0);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (in(k)) rows::store<T, VEC>(to + k * kStep, from[k]);
+  }
+  // All threads have put their numbers of a round of rows: writes a chunk of output `a` to memory.
+  __device__ __forceinline__ void send(const Params& P, int a, T* array, int64_t row) const {
+    const int64_t first = row - team, rest = P.rows - first;
+    T* to = array + first * B.length;
+    const int shift = shift_of(to), end = shift + static_cast<int>((rest < teams ? rest : teams) * B.length * sizeof(T));
+    unsigned char* base = reinterpret_cast<unsigned char*>(to) - shift;
+    const unsigned char* from = chunk(kStages * IN + a);
+    for (int i = threadIdx.x * 16; i < end; i += blockDim.x * 16) {
+      if (i >= shift && i + 16 <= end) {
+        *reinterpret_cast<uint4*>(base + i) = *reinterpret_cast<const uint4*>(from + i);
+      } else {
+        for (int j = i; j < i + 16; j += static_cast<int>(sizeof(T)))
+          if (j >= shift && j < end) *reinterpret_cast<T*>(base + j) = *reinterpret_cast<const T*>(from + j);
+      }
+    }
+  }
+
+  // Sums over the threads of a row.
+  template <int V>
+  __device__ __forceinline__ void sum(A (&v)[V]) {
+#pragma unroll
+    for (int off = LANES >> 1; off; off >>= 1)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    if (LANES < 32 || warps == 1) return;
+    // Two buffers by turns: who writes the first one again has passed the barrier after which nobody reads it.
+    A* at = exchange + turn * (blockDim.x >> 5) * kMaxSums + team * warps * kMaxSums;
+    turn ^= 1;
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < V; ++i) at[warp * kMaxSums + i] = v[i];
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(B.lanes) : "memory");
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = at[i];
+    for (int other = 1; other < warps; ++other)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += at[other * kMaxSums + i];
+  }
+
+  // The sums of the CTA's rows for one array, a number for each channel, written as one row of partial sums.  All threads have left their rows.
+  __device__ __forceinline__ void store_partial(A (&sums)[K][VEC], A* tile, A* __restrict__ to) const {
+#pragma unroll
+    for (int off = LANES; off < 32; off <<= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) sums[k][c] += __shfl_xor_sync(0xffffffffu, sums[k][c], off);
+    const int groups = LANES < 32 ? blockDim.x >> 5 : teams, group = LANES < 32 ? threadIdx.x >> 5 : team;
+    __syncthreads();
+    if ((threadIdx.x & 31) < LANES) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (in(k))
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) tile[group * B.length + column(k) + c] = sums[k][c];
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < B.channels; u += blockDim.x) {
+      A sum = A(0);
+      if (B.components == 1) {
+#pragma unroll 4
+        for (int other = 0; other < groups; ++other) sum += tile[other * B.length + u];
+      } else {
+        for (int m = 0; m < B.components; ++m)
+#pragma unroll 4
+          for (int other = 0; other < groups; ++other) sum += tile[other * B.length + u * B.components + m];
+      }
+      to[u] = sum;
+    }
+  }
+};
+
+// Calls `f` with the number of a warp's threads that share a row of `B`, as a constant.
+template <int THREADS, typename F>
+__device__ __forceinline__ void with_lanes(const Block& B, F&& f) {
+  if constexpr (THREADS > kThreads) {
+    f(std::integral_constant<int, 32>());
+  } else {
+    switch (B.lanes) {
+      case 1: f(std::integral_constant<int, 1>()); break;
+      case 2: f(std::integral_constant<int, 2>()); break;
+      case 4: f(std::integral_constant<int, 4>()); break;
+      case 8: f(std::integral_constant<int, 8>()); break;
+      case 16: f(std::integral_constant<int, 16>()); break;
+      default: f(std::integral_constant<int, 32>()); break;
+    }
+  }
+}
+
+template <typename T>
+struct Operands {
+  const T *x, *weight, *bias, *g, *rx, *rw, *rb;
+  const Moments<Acc<T>>* stats_in;
+  T *y, *gx, *hx, *hg;
+  Moments<Acc<T>>* stats_out;
+  Acc<T>* partial;
+};
+
+template <typename T, int VEC, int K, int LANES, int MODE>
+__device__ __forceinline__ void forward(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
+  using A = Acc<T>;
+  Place<T, VEC, K, LANES, MODE, 1, 1> place(B, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
+  const T* const arrays[1] = {o.x};
+  auto request = [&](int64_t row) { place.request(P, arrays, row); };
+  int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
+  for (int j = 0; j < kStages; ++j) request(row + j * step);
   A w[K][VEC], b[K][VEC];
-  columns.parameters(weight, B.weight_offset, B.components, A(1), w);
-  columns.parameters(B.scalar ? bias : nullptr, B.bias_offset, B.components, A(0), b);
-  const A share = static_cast<A>(B.share), eps = static_cast<A>(P.eps);
-  const int64_t step = static_cast<int64_t>(B.ctas) * team.teams;
-  const int64_t first = static_cast<int64_t>(blockIdx.x - B.first_cta) * team.teams;
-  const int64_t block_index = &B - P.block;
-  for (int64_t base = first; base + team.teams_before_warp() < P.rows; base += step) {
-    const int64_t row = base + team.index;
-    const bool active = row < P.rows;
+  place.parameters(o.weight, B.weight_offset, A(1), w);
+  place.parameters(B.scalar ? o.bias : nullptr, B.bias_offset, A(0), b);
+  const A share = static_cast<A>(B.share), eps = static_cast<A>(P.eps), per_mean = A(1) / static_cast<A>(B.length);
+  for (; row - place.ahead() < P.rows; row += step) {
     A v[K][VEC];
-    columns.load(x + row * P.dim + B.offset, active, v);
+    place.wait();
+    place.take(P, 0, o.x, row, v);
     A mean = A(0);
     if (B.scalar) {
       A sums[1] = {A(0)};
@@ -149,269 +306,257 @@ forward_kernel(const __grid_constant__ Params P, const T* __restrict__ x, const 
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int c = 0; c < VEC; ++c) sums[0] += v[k][c];
-      team.sum(sums);
-      mean = sums[0] / static_cast<A>(B.length);
+      place.sum(sums);
+      mean = sums[0] * per_mean;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) v[k][c] = columns.in(k) ? v[k][c] - mean : A(0);
+        for (int c = 0; c < VEC; ++c) v[k][c] = place.in(k) ? v[k][c] - mean : A(0);
     }
     A sums[1] = {A(0)};
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) sums[0] += v[k][c] * v[k][c];
-    team.sum(sums);
-    const A scale = A(1) / sqrt(sums[0] * share + eps);
-    if (active) {
-      T* to = y + row * P.dim + B.offset;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (columns.in(k)) {
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) v[k][c] = v[k][c] * scale * w[k][c] + b[k][c];
-          rows::store<T, VEC>(to + columns.at(k), v[k]);
-        }
-      if (stats && team.lane == 0) stats[block_index * P.rows + row] = Moments<A>{mean, scale};
-    }
-  }
-}
-
-// The sums of a CTA's teams for one array, written as one row of partial sums.
-template <typename A, int VEC, int K>
-__device__ __forceinline__ void store_partial(const Block& B, Team<A>& team, A (&sums)[K][VEC], A* tile, A* __restrict__ to) {
-  for (int off = team.lanes; off < 32; off <<= 1)
+    place.sum(sums);
+    if (MODE == kPackets) request(row + kStages * step);  // the thread's numbers of this row have gone into the sum
+    const A scale = rsqrt(sums[0] * share + eps);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) sums[k][c] += __shfl_xor_sync(0xffffffffu, sums[k][c], off);
-  const int groups = team.lanes < 32 ? blockDim.x >> 5 : team.teams;
-  const int group = team.lanes < 32 ? threadIdx.x >> 5 : team.index;
-  if ((threadIdx.x & 31) < team.lanes) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int at = (k * team.lanes + team.lane) * VEC;
-      if (at < B.length)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) tile[group * B.length + at + c] = sums[k][c];
+      for (int c = 0; c < VEC; ++c) v[k][c] = v[k][c] * scale * w[k][c] + b[k][c];
+    place.put(P, 0, o.y, row, v);
+    if (MODE == kChunks) {
+      __syncthreads();
+      place.send(P, 0, o.y, row);
+      request(row + kStages * step);
     }
+    if (row < P.rows && o.stats_out && place.lane == 0 && place.warp == 0) o.stats_out[index * P.rows + row] = Moments<A>{mean, scale};
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < B.length; i += blockDim.x) {
-    A sum = tile[i];
-    for (int other = 1; other < groups; ++other) sum += tile[other * B.length + i];
-    to[i] = sum;
-  }
-  __syncthreads();
 }
 
-template <typename T, int VEC, int K, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-backward_kernel(const __grid_constant__ Params P, const T* __restrict__ x, const T* __restrict__ weight,
-                const Moments<Acc<T>>* __restrict__ stats, const T* __restrict__ g, T* __restrict__ gx,
-                Acc<T>* __restrict__ partial) {
+template <typename T, int VEC, int K, int LANES, int MODE>
+__device__ __forceinline__ void backward(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
   using A = Acc<T>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ A exchange[2 * (THREADS / 32) * Team<A>::kMaxSums];
-  const Block& B = block_of(P);
-  Team<A> team(B.lanes, exchange);
-  const Columns<T, VEC, K> columns(B, team.lane);
+  Place<T, VEC, K, LANES, MODE, 2, 1> place(B, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
+  const T* const arrays[2] = {o.x, o.g};
+  auto request = [&](int64_t row) { place.request(P, arrays, row); };
+  auto moments = [&](int64_t row) { return row < P.rows ? o.stats_in[index * P.rows + row] : Moments<A>{A(0), A(0)}; };
+  int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
+  for (int j = 0; j < kStages; ++j) request(row + j * step);
+  Moments<A> next = moments(row);  // a row ahead
   A w[K][VEC], gw[K][VEC], gb[K][VEC];
-  columns.parameters(weight, B.weight_offset, B.components, A(1), w);
+  place.parameters(o.weight, B.weight_offset, A(1), w);
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int c = 0; c < VEC; ++c) gw[k][c] = gb[k][c] = A(0);
-  const A share = static_cast<A>(B.share);
-  const int64_t step = static_cast<int64_t>(B.ctas) * team.teams;
-  const int64_t first = static_cast<int64_t>(blockIdx.x - B.first_cta) * team.teams;
-  const int64_t block_index = &B - P.block;
-  for (int64_t base = first; base + team.teams_before_warp() < P.rows; base += step) {
-    const int64_t row = base + team.index;
-    const bool active = row < P.rows;
+  const A share = static_cast<A>(B.share), per_mean = B.scalar ? A(1) / static_cast<A>(B.length) : A(0);
+  for (; row - place.ahead() < P.rows; row += step) {
     A h[K][VEC], e[K][VEC];
-    columns.load(x + row * P.dim + B.offset, active, h);
-    columns.load(g + row * P.dim + B.offset, active, e);
-    Moments<A> m{A(0), A(0)};
-    if (active) m = stats[block_index * P.rows + row];
+    const Moments<A> m = next;
+    next = moments(row + step);
+    place.wait();
+    place.take(P, 0, o.x, row, h);
+    place.take(P, 1, o.g, row, e);
     A sums[2] = {A(0), A(0)};
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
-        h[k][c] = active && columns.in(k) ? (h[k][c] - m.mean) * m.scale : A(0);
+        // columns that are not there have e = 0: whatever h is, they add nothing, unless the mean is no number
+        h[k][c] = place.in(k) ? (h[k][c] - m.mean) * m.scale : A(0);
         gw[k][c] += e[k][c] * h[k][c];
         gb[k][c] += e[k][c];
         e[k][c] *= w[k][c];
         sums[0] += e[k][c] * h[k][c];
         sums[1] += e[k][c];
       }
-    if (gx) {
-      team.sum(sums);
-      const A along = sums[0] * share, mean = B.scalar ? sums[1] / static_cast<A>(B.length) : A(0);
-      if (active) {
-        T* to = gx + row * P.dim + B.offset;
+    if (o.gx) place.sum(sums);
+    if (MODE == kPackets) request(row + kStages * step);
+    if (o.gx) {
+      const A along = sums[0] * share, mean = sums[1] * per_mean;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (columns.in(k)) {
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int c = 0; c < VEC; ++c) e[k][c] = m.scale * (e[k][c] - mean - h[k][c] * along);
-            rows::store<T, VEC>(to + columns.at(k), e[k]);
-          }
-      }
+        for (int c = 0; c < VEC; ++c) e[k][c] = m.scale * (e[k][c] - mean - h[k][c] * along);
+      place.put(P, 0, o.gx, row, e);
+    }
+    if (MODE == kChunks) {
+      __syncthreads();
+      if (o.gx) place.send(P, 0, o.gx, row);
+      request(row + kStages * step);
     }
   }
-  if (!partial) return;
-  A* to = partial + B.partial + static_cast<int64_t>(blockIdx.x - B.first_cta) * 2 * B.length;
+  if (!o.partial) return;
+  A* to = o.partial + B.partial + static_cast<int64_t>(blockIdx.x - B.first_cta) * 2 * B.channels;
   A* tile = reinterpret_cast<A*>(raw);
-  store_partial(B, team, gw, tile, to);
-  if (B.scalar) store_partial(B, team, gb, tile, to + B.length);
+  wait_copies<0>();
+  place.store_partial(gw, tile, to);
+  if (B.scalar) place.store_partial(gb, tile, to + B.channels);
 }
 
-template <typename T, int VEC, int K, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-second_kernel(const __grid_constant__ Params P, const T* __restrict__ x, const T* __restrict__ weight,
-              const Moments<Acc<T>>* __restrict__ stats, const T* __restrict__ g, const T* __restrict__ rx,
-              const T* __restrict__ rw, const T* __restrict__ rb, T* __restrict__ hx, T* __restrict__ hg,
-              Acc<T>* __restrict__ partial) {
+template <typename T, int VEC, int K, int LANES, int MODE>
+__device__ __forceinline__ void second(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
   using A = Acc<T>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ A exchange[2 * (THREADS / 32) * Team<A>::kMaxSums];
-  const Block& B = block_of(P);
-  Team<A> team(B.lanes, exchange);
-  const Columns<T, VEC, K> columns(B, team.lane);
+  Place<T, VEC, K, LANES, MODE, 3, 2> place(B, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
+  const T* const arrays[3] = {o.x, o.g, o.rx};
+  auto request = [&](int64_t row) { place.request(P, arrays, row); };
+  auto moments = [&](int64_t row) { return row < P.rows ? o.stats_in[index * P.rows + row] : Moments<A>{A(0), A(0)}; };
+  int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
+  for (int j = 0; j < kStages; ++j) request(row + j * step);
+  Moments<A> next = moments(row);
   A w[K][VEC], hw[K][VEC];
-  columns.parameters(weight, B.weight_offset, B.components, A(1), w);
+  place.parameters(o.weight, B.weight_offset, A(1), w);
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int c = 0; c < VEC; ++c) hw[k][c] = A(0);
-  const A share = static_cast<A>(B.share);
-  const int64_t step = static_cast<int64_t>(B.ctas) * team.teams;
-  const int64_t first = static_cast<int64_t>(blockIdx.x - B.first_cta) * team.teams;
-  const int64_t block_index = &B - P.block;
   // rw and rb are as short as a row and the same for all of them: read again from cache instead of kept
   auto other = [&](const T* __restrict__ p, int offset, int k, int c) {
-    return p ? rows::widen(p[offset + (columns.at(k) + c) / B.components]) : A(0);
+    return p && place.in(k) ? rows::widen(p[offset + place.channel(place.column(k) + c)]) : A(0);
   };
-  for (int64_t base = first; base + team.teams_before_warp() < P.rows; base += step) {
-    const int64_t row = base + team.index;
-    const bool active = row < P.rows;
+  const A share = static_cast<A>(B.share), length = static_cast<A>(B.length), per_mean = B.scalar ? A(1) / length : A(0);
+  for (; row - place.ahead() < P.rows; row += step) {
     A h[K][VEC], e[K][VEC], r[K][VEC];
-    columns.load(x + row * P.dim + B.offset, active, h);
-    columns.load(g + row * P.dim + B.offset, active, e);
-    columns.load(rx ? rx + row * P.dim + B.offset : nullptr, active && rx, r);
-    Moments<A> m{A(0), A(0)};
-    if (active) m = stats[block_index * P.rows + row];
+    const Moments<A> m = next;
+    next = moments(row + step);
+    place.wait();
+    place.take(P, 0, o.x, row, h);
+    place.take(P, 1, o.g, row, e);
+    place.take(P, 2, o.rx, row, r);
     A sums[5] = {A(0), A(0), A(0), A(0), A(0)}, more[2] = {A(0), A(0)};  // rh, ch, rc, r, c; q, qh
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
-        h[k][c] = active && columns.in(k) ? (h[k][c] - m.mean) * m.scale : A(0);
+        h[k][c] = place.in(k) ? (h[k][c] - m.mean) * m.scale : A(0);
         const A scaled = e[k][c] * w[k][c];
         sums[0] += r[k][c] * h[k][c];
         sums[1] += scaled * h[k][c];
         sums[2] += r[k][c] * scaled;
         sums[3] += r[k][c];
         sums[4] += scaled;
-        if (rw && columns.in(k)) {
-          const A q = other(rw, B.weight_offset, k, c) * e[k][c];
+        if (o.rw) {
+          const A q = other(o.rw, B.weight_offset, k, c) * e[k][c];
           more[0] += q;
           more[1] += q * h[k][c];
         }
       }
-    team.sum(sums);
-    if (rw) team.sum(more);
-    const A length = static_cast<A>(B.length);
-    const A mean_r = B.scalar ? sums[3] / length : A(0), mean_c = B.scalar ? sums[4] / length : A(0);
-    const A mean_q = B.scalar ? more[0] / length : A(0);
+    place.sum(sums);
+    if (o.rw) place.sum(more);
+    if (MODE == kPackets) request(row + kStages * step);
+    const A mean_r = sums[3] * per_mean, mean_c = sums[4] * per_mean, mean_q = more[0] * per_mean;
     const A dot = sums[2] - length * mean_r * mean_c;
     const A along_r = share * sums[0], along_c = share * sums[1], along_q = share * more[1];
     const A outer = m.scale * m.scale * share, on_h = dot - share * sums[0] * sums[1];
-    if (active) {
-      const int64_t at = row * P.dim + B.offset;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (columns.in(k)) {
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) {
-            const A p = r[k][c] - mean_r - h[k][c] * along_r;
-            const A scaled = e[k][c] * w[k][c] - mean_c - h[k][c] * along_c;
-            const A tangent = rw ? other(rw, B.weight_offset, k, c) : A(0);
-            const A q = rw ? tangent * e[k][c] - mean_q - h[k][c] * along_q : A(0);
-            hw[k][c] += m.scale * p * e[k][c];
-            e[k][c] = w[k][c] * m.scale * p + tangent * h[k][c] + (B.scalar ? other(rb, B.bias_offset, k, c) : A(0));
-            r[k][c] = m.scale * q - outer * (on_h * h[k][c] + sums[1] * p + sums[0] * scaled);
-          }
-          if (hg) rows::store<T, VEC>(hg + at + columns.at(k), e[k]);
-          if (hx) rows::store<T, VEC>(hx + at + columns.at(k), r[k]);
+      for (int c = 0; c < VEC; ++c) {
+        const A p = r[k][c] - mean_r - h[k][c] * along_r;
+        const A scaled = e[k][c] * w[k][c] - mean_c - h[k][c] * along_c;
+        const A from_q = on_h * h[k][c] + sums[1] * p + sums[0] * scaled;
+        hw[k][c] += m.scale * p * e[k][c];  // nothing where there is no column: e is zero
+        A hx = -outer * from_q, hg = w[k][c] * m.scale * p;
+        if (o.rw) {
+          const A tangent = other(o.rw, B.weight_offset, k, c);
+          hx += m.scale * (tangent * e[k][c] - mean_q - h[k][c] * along_q);
+          hg += tangent * h[k][c];
         }
+        if (o.rb && B.scalar) hg += other(o.rb, B.bias_offset, k, c);
+        r[k][c] = hx;
+        e[k][c] = hg;
+      }
+    place.put(P, 0, o.hx, row, r);
+    place.put(P, 1, o.hg, row, e);
+    if (MODE == kChunks) {
+      __syncthreads();
+      if (o.hx) place.send(P, 0, o.hx, row);
+      if (o.hg) place.send(P, 1, o.hg, row);
+      request(row + kStages * step);
     }
   }
-  if (!partial) return;
-  store_partial(B, team, hw, reinterpret_cast<A*>(raw), partial + B.partial + static_cast<int64_t>(blockIdx.x - B.first_cta) * 2 * B.length);
+  if (!o.partial) return;
+  wait_copies<0>();
+  place.store_partial(hw, reinterpret_cast<A*>(raw), o.partial + B.partial + static_cast<int64_t>(blockIdx.x - B.first_cta) * 2 * B.channels);
 }
 
-// The sums of all CTAs, for 32 channels of a block by one CTA: 16 threads take every sixteenth CTA's sums of a channel each.
-constexpr int kFinalSlices = 16;
+enum Order { kForward, kBackward, kSecond };
+
+template <typename T, int VEC, int K, int THREADS, int MODE, int ORDER>
+__global__ void __launch_bounds__(THREADS)
+norm_kernel(const __grid_constant__ Params P, const __grid_constant__ Operands<T> o) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ Acc<T> exchange[2 * (THREADS / 32) * kMaxSums];
+  const int index = block_index_of(P);
+  const Block& B = P.block[index];
+  with_lanes<THREADS>(B, [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    if constexpr (ORDER == kForward) forward<T, VEC, K, LANES, MODE>(P, B, index, o, raw, exchange);
+    if constexpr (ORDER == kBackward) backward<T, VEC, K, LANES, MODE>(P, B, index, o, raw, exchange);
+    if constexpr (ORDER == kSecond) second<T, VEC, K, LANES, MODE>(P, B, index, o, raw, exchange);
+  });
+}
+
+// The sums of all CTAs: 32 channels of a block, for the weights or for the biases, by one CTA, 32 threads for each channel.
+constexpr int kFinalSlices = 32;
 template <typename T>
 __global__ void __launch_bounds__(32 * kFinalSlices)
 final_kernel(const __grid_constant__ Params P, const Acc<T>* __restrict__ partial, T* __restrict__ gw, T* __restrict__ gb) {
   using A = Acc<T>;
-  __shared__ A tile[2][kFinalSlices][32];
+  __shared__ A tile[kFinalSlices][33];
   wait_for_previous();
-  int i = 0, cta = blockIdx.x;  // which block, and which 32 of its channels
-  auto channels = [&](int j) { return P.block[j].length / P.block[j].components; };
-  while (cta >= (channels(i) + 31) / 32) cta -= (channels(i++) + 31) / 32;
+  int i = 0, task = blockIdx.x;  // which block, and which 32 of its channels
+  while (task >= (P.block[i].channels + 31) / 32) task -= (P.block[i++].channels + 31) / 32;
   const Block& B = P.block[i];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, u = cta * 32 + lane, count = channels(i);
-  A sum[2] = {A(0), A(0)};
-  if (u < count) {
-    const A* from = partial + B.partial + static_cast<int64_t>(u) * B.components;
-    for (int j = slice; j < B.ctas; j += kFinalSlices) {
-      const A* row = from + static_cast<int64_t>(j) * 2 * B.length;
-      if (gw)
-        for (int m = 0; m < B.components; ++m) sum[0] += row[m];
-      if (gb && B.scalar) sum[1] += row[B.length];
-    }
+  const bool biases = blockIdx.y;
+  T* to = biases ? gb : gw;
+  if (!to || (biases && !B.scalar)) return;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, first = task * 32;
+  A sum = A(0);
+  if (first + lane < B.channels) {
+    const A* column = partial + B.partial + (biases ? B.channels : 0) + first + lane;
+    const int64_t stride = 2 * static_cast<int64_t>(B.channels);
+#pragma unroll 8
+    for (int j = slice; j < B.ctas; j += kFinalSlices) sum += column[j * stride];
   }
-  tile[0][slice][lane] = sum[0];
-  tile[1][slice][lane] = sum[1];
+  tile[slice][lane] = sum;
   __syncthreads();
-  if (slice >= 2 || u >= count) return;
-  A total = A(0);
-#pragma unroll
-  for (int j = 0; j < kFinalSlices; ++j) total += tile[slice][j][lane];
-  if (slice == 0 && gw) rows::narrow(total, gw[B.weight_offset + u]);
-  if (slice == 1 && gb && B.scalar) rows::narrow(total, gb[B.bias_offset + u]);
+  A total = tile[lane][slice];  // a warp's threads have the slices of one channel
+  for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  if (lane == 0 && first + slice < B.channels) rows::narrow(total, to[(biases ? B.bias_offset : B.weight_offset) + first + slice]);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------
 
-struct Operands {
+struct Call {
   const void *x, *weight, *bias, *stats_in, *g, *rx, *rw, *rb;
   void *y, *stats_out, *gx, *gw, *gb, *hx, *hg;
   void* scratch;
   int64_t scratch_bytes;
 };
-enum Order { kForward, kBackward, kSecond };
 
-inline int blocks_on_device(const void* kernel, int threads, size_t shared) {
-  int resident = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, shared) != cudaSuccess || resident < 1) resident = 1;
-  return resident * rows::processors();
-}
-
-// Gives every block its threads per row and its CTAs: as many as its rows want, or its share of the resident ones.
-inline int assign(Params& P, int vec, int packets, int threads, int resident) {
-  int64_t wanted = 0;
+// Gives every block its threads per row; returns the largest chunk.
+template <typename T>
+int lay_out(Params& P, int vec, int packets, int threads) {
+  int most = 0;
   for (int i = 0; i < P.blocks; ++i) {
     Block& B = P.block[i];
     B.lanes = rows::next_power_of_two(ceil_div(ceil_div(B.length, vec), packets));
-    if (B.lanes > 32 && threads / B.lanes > 15) B.lanes = threads / 8;  // a CTA has fifteen barriers beside its own
-    wanted += ceil_div(P.rows, threads / B.lanes);
+    if (threads > kThreads && B.lanes < 128) B.lanes = 128;  // a CTA has fifteen barriers beside its own
+    B.chunk = (threads / B.lanes * B.length * static_cast<int>(sizeof(T)) + 15) / 16 * 16 + 16;  // beginning anywhere in a piece
+    most = most < B.chunk ? B.chunk : most;
   }
+  return most;
+}
+
+// Gives every block its CTAs: as many as its rows want, or its share of the resident ones.
+inline int assign(Params& P, int threads, int resident) {
+  int64_t wanted = 0;
+  for (int i = 0; i < P.blocks; ++i) wanted += ceil_div(P.rows, threads / P.block[i].lanes);
   int ctas = 0;
   int64_t partial = 0;
   for (int i = 0; i < P.blocks; ++i) {
@@ -425,63 +570,54 @@ inline int assign(Params& P, int vec, int packets, int threads, int resident) {
     B.ctas = static_cast<int>(count);
     B.partial = partial;
     ctas += B.ctas;
-    partial += count * 2 * B.length;
+    partial += count * 2 * B.channels;
   }
   return ctas;
 }
-constexpr int kThreads = 256, kWideThreads = 1024;
 // At most this many CTAs of kThreads are resident on a multiprocessor, whatever a kernel needs.
 constexpr int kMostResident = 2048 / kThreads;
-
 inline int64_t scratch_elements(const Params& P) {
   const int64_t resident = static_cast<int64_t>(kMostResident) * rows::processors();
   return (P.rows < resident ? P.rows : resident) * 2 * P.dim + 2;  // never zero: a buffer of no bytes has no address
 }
 
-template <typename T, int VEC, int K, int THREADS>
-int launch(Order order, Params P, const Operands& o, cudaStream_t stream) {
+template <typename T, int VEC, int K, int THREADS, int MODE, int ORDER>
+int launch(Params P, const Call& c, cudaStream_t stream) {
   using A = Acc<T>;
   auto in = [](const void* p) { return static_cast<const T*>(p); };
   auto out = [](void* p) { return static_cast<T*>(p); };
-  const Moments<A>* stats = static_cast<const Moments<A>*>(o.stats_in);
-  // Room for the sums of the CTA's threads: at most all of them
-  const size_t shared = order == kForward ? 0 : static_cast<size_t>(THREADS) * K * VEC * sizeof(A);
-  const bool sums = order != kForward && (o.gw || o.gb);
-  const void* kernel = order == kForward    ? reinterpret_cast<const void*>(forward_kernel<T, VEC, K, THREADS>)
-                       : order == kBackward ? reinterpret_cast<const void*>(backward_kernel<T, VEC, K, THREADS>)
-                                            : reinterpret_cast<const void*>(second_kernel<T, VEC, K, THREADS>);
-  if (shared > 48 * 1024) LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
-  static std::atomic<int> known[3];
-  int resident = known[order].load(std::memory_order_relaxed);
-  if (!resident) {
-    resident = blocks_on_device(kernel, THREADS, shared);
-    if (resident < 1) return fail(LUNA_ERR_CUDA, "the current device's multiprocessors are unknown");
-    known[order].store(resident, std::memory_order_relaxed);
-  }
-  const int ctas = assign(P, VEC, K, THREADS, resident);
-  A* partial = sums ? static_cast<A*>(o.scratch) : nullptr;
+  const bool sums = ORDER != kForward && (c.gw || c.gb);
+  // Room for the rows on their way and on their way out, and later for the sums of the CTA's threads
+  constexpr int in_arrays = ORDER == kForward ? 1 : ORDER == kBackward ? 2 : 3, out_arrays = ORDER == kSecond ? 2 : 1;
+  const size_t chunk = lay_out<T>(P, VEC, K, THREADS);
+  const size_t rows_bytes = MODE == kDirect ? 0 : MODE == kPackets ? kStages * in_arrays * K * THREADS * 16 : (kStages * in_arrays + out_arrays) * chunk;
+  const size_t sums_bytes = sums ? static_cast<size_t>(THREADS) * K * VEC * sizeof(A) : 0;
+  const size_t shared = rows_bytes > sums_bytes ? rows_bytes : sums_bytes;
+  const auto kernel = norm_kernel<T, VEC, K, THREADS, MODE, ORDER>;
+  if (shared > 40 * 1024) LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+  int resident = 0;
+  LUNA_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, THREADS, shared));
+  resident *= rows::processors();
+  if (resident < 1) return fail(LUNA_ERR_CUDA, "layer norm does not fit the current device");
+  const int ctas = assign(P, THREADS, resident);
+  const Operands<T> o{in(c.x), in(c.weight), in(c.bias), in(c.g), in(c.rx), in(c.rw), in(c.rb), static_cast<const Moments<A>*>(c.stats_in),
+                      out(c.y), out(c.gx), out(c.hx), out(c.hg), static_cast<Moments<A>*>(c.stats_out),
+                      sums ? static_cast<A*>(c.scratch) : nullptr};
   if (ctas > 0) {
-    if (order == kForward)
-      forward_kernel<T, VEC, K, THREADS><<<ctas, THREADS, 0, stream>>>(P, in(o.x), in(o.weight), in(o.bias), out(o.y),
-                                                                       static_cast<Moments<A>*>(o.stats_out));
-    else if (order == kBackward)
-      backward_kernel<T, VEC, K, THREADS><<<ctas, THREADS, shared, stream>>>(P, in(o.x), in(o.weight), stats, in(o.g), out(o.gx), partial);
-    else
-      second_kernel<T, VEC, K, THREADS><<<ctas, THREADS, shared, stream>>>(P, in(o.x), in(o.weight), stats, in(o.g), in(o.rx), in(o.rw),
-                                                                           in(o.rb), out(o.hx), out(o.hg), partial);
+    kernel<<<ctas, THREADS, shared, stream>>>(P, o);
     LUNA_LAUNCH_CHECK("layer norm");
   }
   if (sums) {
     int tasks = 0;
-    for (int i = 0; i < P.blocks; ++i) tasks += static_cast<int>(ceil_div(P.block[i].length / P.block[i].components, 32));
-    launch_early(final_kernel<T>, dim3(tasks), 32 * kFinalSlices, 0, stream, P, static_cast<const A*>(partial), out(o.gw), out(o.gb));
+    for (int i = 0; i < P.blocks; ++i) tasks += (P.block[i].channels + 31) / 32;
+    launch_early(final_kernel<T>, dim3(tasks, c.gb ? 2 : 1), 32 * kFinalSlices, 0, stream, P, static_cast<const A*>(o.partial), out(c.gw), out(c.gb));
     LUNA_LAUNCH_CHECK("sums of the layer norm");
   }
   return LUNA_OK;
 }
 
-template <typename T>
-int run(Order order, const Params& P, const Operands& o, cudaStream_t stream) {
+template <typename T, int ORDER>
+int choose(const Params& P, const Call& c, cudaStream_t stream) {
   constexpr int kPacket = 16 / static_cast<int>(sizeof(T));
   bool packets = P.dim % kPacket == 0;
   int64_t longest = 0;
@@ -489,26 +625,41 @@ int run(Order order, const Params& P, const Operands& o, cudaStream_t stream) {
     packets = packets && P.block[i].offset % kPacket == 0 && P.block[i].length % kPacket == 0;
     longest = P.block[i].length > longest ? P.block[i].length : longest;
   }
-  for (const void* p : {o.x, o.g, o.rx, static_cast<const void*>(o.y), static_cast<const void*>(o.gx), static_cast<const void*>(o.hx),
-                        static_cast<const void*>(o.hg)})
+  for (const void* p : {c.x, c.g, c.rx, static_cast<const void*>(c.y), static_cast<const void*>(c.gx), static_cast<const void*>(c.hx),
+                        static_cast<const void*>(c.hg)})
     packets = packets && aligned_to(p, 16);
+  // Packets of a thread.  More of them mean fewer threads per row, so fewer steps for its sums and no barrier, as long as the
+  // registers allow it.  Measured, forward / backward / second order in us: 50,000 rows of 128x0e+128x1o+128x2e, FP32, one, two
+  // or four packets 139 / 199, 87 / 168, 84 / 123; 100,000 of 64x0e+64x1o+64x2e 139 / 180 / 336, 86 / 163 / 235, 82 / 123 / 287;
+  // 86,000 of 64x0e 10.9 / 13.0, 8.9 / 14.9, 9.7 / 15.4; 40,000 of 1024x0e, BF16, 58 / 76, 55 / 63, 54 / 79.  Where there are not
+  // enough rows to fill the GPU, the threads are: 24 rows 2.6, 2.8 and 3.6 us, 500 rows of 64x0e 2.6 / 3.1, 3.1 / 4.2, 4.0 / 5.7.
+  const bool few = P.rows * P.dim <= static_cast<int64_t>(rows::processors()) * 1024 * (packets ? kPacket : 1);
   if (packets) {
     const int64_t n = longest / kPacket;
-    if (n <= 32) return launch<T, kPacket, 1, kThreads>(order, P, o, stream);
-    if (n <= 64) return launch<T, kPacket, 2, kThreads>(order, P, o, stream);
-    if (n <= kThreads * 4) return launch<T, kPacket, 4, kThreads>(order, P, o, stream);
-    if (n <= kWideThreads * 4) return launch<T, kPacket, 4, kWideThreads>(order, P, o, stream);
+    const int64_t most_of_two = ORDER == kSecond || sizeof(T) == 2 ? kThreads * 2 : 64;
+    if (few && n <= kThreads) return launch<T, kPacket, 1, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= most_of_two) return launch<T, kPacket, 2, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= kThreads * 4) return launch<T, kPacket, 4, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= kWideThreads * 4) return launch<T, kPacket, 4, kWideThreads, kDirect, ORDER>(P, c, stream);
   }
-  if (longest <= 32) return launch<T, 1, 1, kThreads>(order, P, o, stream);
-  if (longest <= kThreads * 4) return launch<T, 1, 4, kThreads>(order, P, o, stream);
-  if (longest <= kThreads * 16) return launch<T, 1, 16, kThreads>(order, P, o, stream);
-  return launch<T, 1, 16, kWideThreads>(order, P, o, stream);
+  constexpr int kMost = sizeof(T) > 4 ? 8 : 16;  // numbers of a thread
+  if (longest <= kThreads * kMost) {
+    if (P.blocks > 1) return launch<T, 1, kMost, kThreads, kDirect, ORDER>(P, c, stream);
+    if (few && longest <= kThreads * 4) return launch<T, 1, 4, kThreads, kChunks, ORDER>(P, c, stream);
+    return launch<T, 1, kMost, kThreads, kChunks, ORDER>(P, c, stream);
+  }
+  return launch<T, 1, 16, kWideThreads, kDirect, ORDER>(P, c, stream);
 }
 
-extern template int run<float>(Order, const Params&, const Operands&, cudaStream_t);
-extern template int run<double>(Order, const Params&, const Operands&, cudaStream_t);
-extern template int run<rows::bf16>(Order, const Params&, const Operands&, cudaStream_t);
-extern template int run<rows::f16>(Order, const Params&, const Operands&, cudaStream_t);
+template <typename T>
+int run(Order order, const Params& P, const Call& c, cudaStream_t stream) {
+  return order == kForward ? choose<T, kForward>(P, c, stream) : order == kBackward ? choose<T, kBackward>(P, c, stream) : choose<T, kSecond>(P, c, stream);
+}
+
+extern template int run<float>(Order, const Params&, const Call&, cudaStream_t);
+extern template int run<double>(Order, const Params&, const Call&, cudaStream_t);
+extern template int run<rows::bf16>(Order, const Params&, const Call&, cudaStream_t);
+extern template int run<rows::f16>(Order, const Params&, const Call&, cudaStream_t);
 
 }  // namespace norm
 }  // namespace luna

@@ -1,4 +1,4 @@
 #include "layer_norm.cuh"
 namespace luna::norm {
-template int run<rows::f16>(Order, const Params&, const Operands&, cudaStream_t);
+template int run<rows::f16>(Order, const Params&, const Call&, cudaStream_t);
 }

@@ -137,14 +137,17 @@ class LunaTPGraph:
         return holder
 
     def row_holder(self):
-        """The rows of in-edges for the C++ launch path, long ones cut into pieces (``split_rows``)."""
+        """The rows of in-edges for the C++ launch path, long ones cut into pieces of ``ROW_SPLIT_EDGES`` edges."""
         holder = self._tables.get("rows")
         if holder is None:
-            split = self.split_rows()
-            cut = split is not None and split.destinations.virtual_rows > self.num_nodes
-            holder = self._tables["rows"] = _native.binding().Rows(
-                split.graph.dst_rowptr if cut else self.dst_rowptr, self.num_edges,
-                split.destinations.first if cut else None, split.destinations.rows if cut else None)
+            rowptr, first, node = self.dst_rowptr, None, None
+            if self.can_split and self.num_edges and int(rowptr.diff().max()) > ROW_SPLIT_EDGES:
+                split = RowSplit(rowptr, ROW_SPLIT_EDGES)
+                first, node = split.first, split.rows
+                piece = torch.arange(split.virtual_rows, device=rowptr.device) - first[node]
+                begin = rowptr[node] + piece * ROW_SPLIT_EDGES
+                rowptr = torch.cat([begin, rowptr[-1:]]).to(torch.int32)
+            holder = self._tables["rows"] = _native.binding().Rows(rowptr, self.num_edges, first, node)
         return holder
 
     def destination_range(self, begin: int, end: int) -> "tuple[LunaTPGraph, int, int]":
