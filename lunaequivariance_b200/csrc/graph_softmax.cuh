@@ -6,10 +6,12 @@
 //   second     the cotangent r of dz, R = sum alpha r:   d/dg = alpha (r - R),   d/dalpha = r (g - D) - g R
 // Where alpha is zero nothing flows, whatever stands in g or r there.
 //
-// Bound by HBM: a row's values are read once and held in registers between its sums and its outputs, as far as they fit; the rest of
-// a longer row is read again from cache.  `lanes` threads of a warp share a row, or a whole CTA where rows are long; of them
-// `across` (a power of two) lie side by side over an edge's heads.  Rows of more than a thousand edges come cut into pieces: one
-// launch makes the pieces' sums, one joins those of each node, and one makes the outputs.
+// Bound by HBM: a row's values are read once and held in registers between its sums and its outputs, as far as they fit (K packets
+// of a thread); the rest of a longer row passes twice, the second time from cache.  All loads of a batch are under way before
+// the first is waited for: with the mask and the table looked up edge by edge, 2.6 M edges with 8 heads took 94 us forward.
+// `lanes` threads of a warp share a row, or a whole CTA where rows are long; of them `across` (a power of two) lie side by side
+// over an edge's heads.  Rows of more than a thousand edges come cut into pieces: one launch makes the pieces' sums, one joins
+// those of each node, and one makes the outputs.
 #pragma once
 
 #include "rows.cuh"
@@ -98,7 +100,7 @@ __device__ __forceinline__ A lowest() {
 }
 
 template <typename T, int VEC, int K, int ORDER, int PHASE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ORDER == kSecond ? 2 : ORDER == kForward ? 3 : 4)
 rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __restrict__ stats) {
   using A = Acc<T>;
   __shared__ A exchange[2 * kThreads * VEC];
@@ -110,65 +112,74 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
   const int teams = kThreads / S.lanes, team = threadIdx.x / S.lanes;
   const int ahead = S.lanes < 32 ? team % (32 / S.lanes) : 0;  // teams of this warp before this one: they leave together
 
-  auto table_row = [&](const T* __restrict__ table, int64_t e, A (&v)[VEC]) {
-    const int b = o.buckets[e];
-    if (b >= 0 && b < S.num_buckets) {
-      rows::load<T, VEC>(table + static_cast<int64_t>(b) * S.heads + head, v);
-    } else {
+  // K edges of a thread: z (forward), or alpha and g and the cotangent r
+  A u[K][VEC], g[K][VEC], r[K][VEC];
+  const T* const table = ORDER == kForward ? o.table : ORDER == kSecond ? o.rtable : nullptr;
+  const int stride = slots * S.heads;
+  using In = rows::Pack<T, VEC>;
+  auto fetch = [&](int64_t first, int64_t end) {
+    In t[K];
+    int bucket[K];
+    bool keep[K];
+    const int left = end - first > K * slots ? K * slots : static_cast<int>(end - first);  // this thread's edges: k * slots < left
+    const int64_t at = first * S.heads + head;
+    auto there = [&](int k) { return k * slots < left; };
+    auto bring = [&](const T* __restrict__ array, A (&to)[K][VEC], A otherwise) {
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) v[c] = A(0);
-    }
-  };
-  // What an edge brings: z (forward), alpha and g, and r.
-  auto fetch = [&](int64_t e, A (&u)[VEC], A (&g)[VEC], A (&r)[VEC]) {
-    if constexpr (ORDER == kForward) {
-      if (o.mask && !o.mask[e]) {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) u[c] = lowest<A>();
-        return;
-      }
-      rows::load<T, VEC>(o.logits + e * S.heads + head, u);
-      if (o.table) {
-        A t[VEC];
-        table_row(o.table, e, t);
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) u[c] += t[c];
-      }
-    } else {
-      rows::load<T, VEC>(o.alpha + e * S.heads + head, u);
-      rows::load<T, VEC>(o.g + e * S.heads + head, g);
-      if constexpr (ORDER == kSecond) {
-        if (o.r) {
-          rows::load<T, VEC>(o.r + e * S.heads + head, r);
+      for (int k = 0; k < K; ++k) {
+        if (there(k)) {
+          rows::load<T, VEC>(array + at + k * stride, to[k]);
         } else {
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) r[c] = A(0);
-        }
-        if (o.rtable) {
-          A t[VEC];
-          table_row(o.rtable, e, t);
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) r[c] += t[c];
+          for (int c = 0; c < VEC; ++c) to[k][c] = otherwise;
         }
       }
-    }
-  };
-  auto put = [&](int64_t e, const A (&u)[VEC], const A (&g)[VEC], const A (&r)[VEC], const A (&a)[VEC], const A (&b)[VEC]) {
-    A v[VEC], w[VEC];
+    };
+    auto nothing = [&](A (&to)[K][VEC]) {
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) {
-      if constexpr (ORDER == kForward) {
-        v[c] = u[c] * b[c];
-      } else if constexpr (ORDER == kBackward) {
-        v[c] = u[c] != A(0) ? u[c] * (g[c] - a[c]) : A(0);
-      } else {
-        v[c] = u[c] != A(0) ? u[c] * (r[c] - b[c]) : A(0);
-        w[c] = u[c] != A(0) ? r[c] * (g[c] - a[c]) - g[c] * b[c] : A(0);
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) to[k][c] = A(0);
+    };
+    if (table) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) bucket[k] = there(k) ? o.buckets[first + k * slots] : -1;
+    }
+    if constexpr (ORDER == kForward) {
+      if (o.mask) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) keep[k] = there(k) && o.mask[first + k * slots];
+      }
+      bring(o.logits, u, lowest<A>());
+    } else {
+      bring(o.alpha, u, A(0));
+      bring(o.g, g, A(0));
+      if constexpr (ORDER == kSecond) {
+        if (o.r)
+          bring(o.r, r, A(0));
+        else
+          nothing(r);
       }
     }
-    if (o.out) rows::store<T, VEC>(o.out + e * S.heads + head, v);
-    if constexpr (ORDER == kSecond) {
-      if (o.out2) rows::store<T, VEC>(o.out2 + e * S.heads + head, w);
+    if (table) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) t[k].a[c] = T(0);
+        if (bucket[k] >= 0 && bucket[k] < S.num_buckets) t[k] = *reinterpret_cast<const In*>(table + static_cast<int64_t>(bucket[k]) * S.heads + head);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) (ORDER == kForward ? u : r)[k][c] += rows::widen(t[k].a[c]);
+    }
+    if constexpr (ORDER == kForward) {
+      if (o.mask) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) u[k][c] = keep[k] ? u[k][c] : lowest<A>();
+      }
     }
   };
 
@@ -179,77 +190,60 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
       begin = R.rowptr[row];
       end = R.rowptr[row + 1];
     }
+    const int64_t batch = static_cast<int64_t>(K) * slots;
+    const int64_t last = begin + slot + (end > begin ? (end - begin - 1) / batch * batch : 0);  // the thread's place in the last batch
     begin += slot;
-    A u[K][VEC], g[K][VEC], r[K][VEC];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t e = begin + k * slots;
-      if (e < end) fetch(e, u[k], g[k], r[k]);
-    }
-    const int64_t rest = begin + static_cast<int64_t>(K) * slots;
     A a[VEC], b[VEC];  // forward: the largest logit and the sum; else D and R
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      a[c] = ORDER == kForward ? lowest<A>() : A(0);
+      b[c] = A(0);
+    }
+    A factor[VEC];  // forward: from the exponentials in registers to alpha
     if constexpr (PHASE != kApply) {
+      // From the last batch to the first, which stays in registers.  Forward: each thread has a largest logit and a sum of its
+      // own, which grow together, and keeps exp(z - its largest).
+      for (int64_t e = last; e >= begin; e -= batch) {
+        fetch(e, end);
+        if constexpr (ORDER == kForward) {
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        a[c] = ORDER == kForward ? lowest<A>() : A(0);
-        b[c] = A(0);
-      }
-      auto take = [&](const A (&p)[VEC], const A (&q)[VEC], const A (&s)[VEC]) {
+          for (int c = 0; c < VEC; ++c) {
+            const A before = a[c];
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) {
-          if constexpr (ORDER == kForward) {
-            a[c] = fmax(a[c], p[c]);
-          } else {
-            a[c] += p[c] != A(0) ? p[c] * q[c] : A(0);
-            if constexpr (ORDER == kSecond) b[c] += p[c] != A(0) ? p[c] * s[c] : A(0);
+            for (int k = 0; k < K; ++k) a[c] = fmax(a[c], u[k][c]);
+            const A shift = a[c] == lowest<A>() ? A(0) : a[c];  // nothing left, or nothing but NaN
+            if (b[c] != A(0)) b[c] *= exponential((before == lowest<A>() ? shift : before) - shift);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              u[k][c] = exponential(u[k][c] - shift);
+              b[c] += u[k][c];
+            }
           }
-        }
-      };
+        } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (begin + k * slots < end) take(u[k], g[k], r[k]);
-      for (int64_t e = rest; e < end; e += slots) {
-        A p[VEC], q[VEC], s[VEC];
-        fetch(e, p, q, s);
-        take(p, q, s);
-      }
-      if constexpr (ORDER == kForward) {
-        together.max(a);
-        A shift[VEC];
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) shift[c] = a[c] == lowest<A>() ? A(0) : a[c];  // nothing left, or nothing but NaN
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (begin + k * slots < end)
+          for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int c = 0; c < VEC; ++c) {
-              const A w = exponential(u[k][c] - shift[c]);
-              if constexpr (PHASE == kWhole) u[k][c] = w;
-              b[c] += w;
+              a[c] += u[k][c] != A(0) ? u[k][c] * g[k][c] : A(0);
+              if constexpr (ORDER == kSecond) b[c] += u[k][c] != A(0) ? u[k][c] * r[k][c] : A(0);
             }
-        for (int64_t e = rest; e < end; e += slots) {
-          A p[VEC], q[VEC], s[VEC];
-          fetch(e, p, q, s);
+        }
+      }
+      if constexpr (ORDER == kForward) {
+        A own[VEC];
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) b[c] += exponential(p[c] - shift[c]);
+        for (int c = 0; c < VEC; ++c) own[c] = a[c];
+        together.max(a);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          const A shift = a[c] == lowest<A>() ? A(0) : a[c];
+          factor[c] = own[c] == lowest<A>() ? A(1) : exponential(own[c] - shift);
+          b[c] *= factor[c];
         }
         together.sum(b);
       } else {
         together.sum(a);
         if constexpr (ORDER == kSecond) together.sum(b);
-      }
-    } else {
-      if (row < R.count && here) {
-        const int64_t at = R.first[R.node[row]] * S.heads + head;
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) {
-          const Pair<A> known = stats[at + c];
-          a[c] = known.a;
-          b[c] = known.b;
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) a[c] = b[c] = A(0);
       }
     }
     if constexpr (PHASE == kSums) {
@@ -257,73 +251,88 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
 #pragma unroll
         for (int c = 0; c < VEC; ++c) stats[row * S.heads + head + c] = Pair<A>{a[c], b[c]};
     } else {
+      if constexpr (PHASE == kApply) {
+        if (row < R.count && here) {
+          const int64_t at = R.first[R.node[row]] * S.heads + head;
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) {
+            const Pair<A> known = stats[at + c];
+            a[c] = known.a;
+            b[c] = known.b;
+          }
+        }
+      }
       if constexpr (ORDER == kForward) {
 #pragma unroll
         for (int c = 0; c < VEC; ++c) {
           a[c] = a[c] == lowest<A>() ? A(0) : a[c];
           b[c] = b[c] == A(0) ? A(0) : A(1) / b[c];
-        }
-        if constexpr (PHASE == kApply) {
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-            if (begin + k * slots < end)
-#pragma unroll
-              for (int c = 0; c < VEC; ++c) u[k][c] = exponential(u[k][c] - a[c]);
+          if constexpr (PHASE == kWhole) factor[c] *= b[c];
         }
       }
+      for (int64_t e = begin; e <= last; e += batch) {
+        if (PHASE == kApply || e > begin) {
+          fetch(e, end);
+          if constexpr (ORDER == kForward) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int64_t e = begin + k * slots;
-        if (e < end) put(e, u[k], g[k], r[k], a, b);
-      }
-      for (int64_t e = rest; e < end; e += slots) {
-        A p[VEC], q[VEC], s[VEC];
-        fetch(e, p, q, s);
-        if constexpr (ORDER == kForward) {
+            for (int c = 0; c < VEC; ++c) {
+              factor[c] = b[c];
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) p[c] = exponential(p[c] - a[c]);
+              for (int k = 0; k < K; ++k) u[k][c] = exponential(u[k][c] - a[c]);
+            }
+          }
         }
-        put(e, p, q, s, a, b);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (e + k * slots >= end) continue;
+          const int64_t at = e * S.heads + head + k * stride;
+          A v[VEC], w[VEC];
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) {
+            const A alpha = u[k][c];
+            if constexpr (ORDER == kForward) {
+              v[c] = alpha * factor[c];
+            } else if constexpr (ORDER == kBackward) {
+              v[c] = alpha != A(0) ? alpha * (g[k][c] - a[c]) : A(0);
+            } else {
+              v[c] = alpha != A(0) ? alpha * (r[k][c] - b[c]) : A(0);
+              w[c] = alpha != A(0) ? r[k][c] * (g[k][c] - a[c]) - g[k][c] * b[c] : A(0);
+            }
+          }
+          if (o.out) rows::store<T, VEC>(o.out + at, v);
+          if constexpr (ORDER == kSecond)
+            if (o.out2) rows::store<T, VEC>(o.out2 + at, w);
+        }
       }
     }
   }
 }
 
-// Joins the sums of the pieces of every node that has several, in its first piece's place: a warp per node.
+// Joins the sums of the pieces of every node that has several, in its first piece's place: a warp per node, `across` of its
+// threads (a power of two) side by side over the heads.
 template <typename A, bool FORWARD>
 __global__ void __launch_bounds__(kThreads)
-join_kernel(const Rows R, int heads, Pair<A>* __restrict__ stats) {
+join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
   const int lane = threadIdx.x & 31;
   const int64_t node = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (node >= R.nodes) return;
   const int64_t first = R.first[node], pieces = (node + 1 < R.nodes ? R.first[node + 1] : R.count) - first;
   if (pieces < 2) return;
-  for (int h = 0; h < heads; ++h) {
-    A a = FORWARD ? lowest<A>() : A(0), b = A(0);
-    for (int64_t p = lane; p < pieces; p += 32) {
-      const Pair<A> piece = stats[(first + p) * heads + h];
-      if (FORWARD) {
-        a = fmax(a, piece.a);
-      } else {
-        a += piece.a;
-        b += piece.b;
-      }
-    }
-    for (int off = 16; off; off >>= 1) {
-      const A other = __shfl_xor_sync(0xffffffffu, a, off);
-      a = FORWARD ? fmax(a, other) : a + other;
-    }
-    if (FORWARD) {
-      const A shift = a == lowest<A>() ? A(0) : a;
-      for (int64_t p = lane; p < pieces; p += 32) {
-        const Pair<A> piece = stats[(first + p) * heads + h];
-        // a piece without a largest logit has nothing (a sum of zero) or nothing but NaN, in its sum too
-        b += piece.a == lowest<A>() ? piece.b : piece.b * exponential(piece.a - shift);
-      }
-    }
-    for (int off = 16; off; off >>= 1) b += __shfl_xor_sync(0xffffffffu, b, off);
+  // one pair after the other; a pair without a largest logit has nothing (a sum of zero), or nothing but NaN, in its sum too
+  auto join = [](Pair<A> p, Pair<A> q) {
+    if (!FORWARD) return Pair<A>{p.a + q.a, p.b + q.b};
+    const A top = fmax(p.a, q.a), shift = top == lowest<A>() ? A(0) : top;
+    return Pair<A>{top, (p.a == lowest<A>() ? p.b : p.b * exponential(p.a - shift)) + (q.a == lowest<A>() ? q.b : q.b * exponential(q.a - shift))};
+  };
+  for (int base = 0; base < heads; base += across) {
+    const int h = base + (lane & (across - 1));
+    Pair<A> sum{FORWARD ? lowest<A>() : A(0), A(0)};
+    if (h < heads)
+      for (int64_t p = lane / across; p < pieces; p += 32 / across) sum = join(sum, stats[(first + p) * heads + h]);
+    for (int off = 16; off >= across; off >>= 1)
+      sum = join(sum, Pair<A>{__shfl_xor_sync(0xffffffffu, sum.a, off), __shfl_xor_sync(0xffffffffu, sum.b, off)});
     __syncwarp();  // all have read the first piece
-    if (lane == 0) stats[first * heads + h] = Pair<A>{a, b};
+    if (lane < across && h < heads) stats[first * heads + h] = sum;
   }
 }
 
@@ -351,7 +360,7 @@ int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, con
   auto* stats = static_cast<Pair<Acc<T>>*>(scratch);
   if (!R.first) return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
   if (const int status = start<T, VEC, K, ORDER, kSums>(R, S, o, stats, stream)) return status;
-  join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(ceil_div(R.nodes, kThreads / 32)), kThreads, 0, stream>>>(R, S.heads, stats);
+  join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(ceil_div(R.nodes, kThreads / 32)), kThreads, 0, stream>>>(R, S.heads, S.across, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges: pieces");
   return start<T, VEC, K, ORDER, kApply>(R, S, o, stats, stream);
 }

@@ -7,32 +7,57 @@ namespace {
 
 // bucket = number of boundaries b with b <= |v|, compared as b |b| <= |v|^2 in double precision: for single precision the
 // squares are exact, so only the two additions round.  Boundaries ascend.  Bound by HBM: 12 (24) bytes in, 4 out.
-constexpr int kSharedBoundaries = 2048;
+// Four edges of a thread are searched for together, in as many steps for all of them.
+constexpr int kSharedBoundaries = 2047;
 template <typename T>
 __global__ void __launch_bounds__(256)
-buckets_kernel(const T* __restrict__ vec, const T* __restrict__ boundaries, int count, int32_t* __restrict__ out, int64_t edges) {
+buckets_kernel(const T* __restrict__ vec, const T* __restrict__ boundaries, int count, int32_t* __restrict__ out, int64_t edges,
+               bool aligned) {
   __shared__ double squares[kSharedBoundaries];
-  const bool shared = count <= kSharedBoundaries;
   auto square = [&](int i) {
     const double b = static_cast<double>(boundaries[i]);
     return __dmul_rn(b, fabs(b));
   };
+  int steps = 1;  // a power of two above the count
+  while (steps <= count) steps <<= 1;
+  const bool shared = count <= kSharedBoundaries;
   if (shared)
-    for (int i = threadIdx.x; i < count; i += blockDim.x) squares[i] = square(i);
+    for (int i = threadIdx.x; i < steps - 1; i += blockDim.x) squares[i] = i < count ? square(i) : __longlong_as_double(-1);  // no number
   __syncthreads();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < edges; e += step) {
-    const double x = vec[e * 3], y = vec[e * 3 + 1], z = vec[e * 3 + 2];
-    const double length = __dadd_rn(__dadd_rn(__dmul_rn(x, x), __dmul_rn(y, y)), __dmul_rn(z, z));
-    int low = 0, high = count;
-    while (low < high) {
-      const int middle = (low + high) >> 1;
-      if ((shared ? squares[middle] : square(middle)) <= length)
-        low = middle + 1;
-      else
-        high = middle;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x * 4;
+  for (int64_t first = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4; first < edges; first += step) {
+    T v[12];
+    if (aligned && first + 4 <= edges) {
+      constexpr int per = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+      for (int i = 0; i < 12 / per; ++i) {
+        const rows::Pack<T, per> p = reinterpret_cast<const rows::Pack<T, per>*>(vec + first * 3)[i];
+#pragma unroll
+        for (int c = 0; c < per; ++c) v[i * per + c] = p.a[c];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 12; ++i) v[i] = first * 3 + i < edges * 3 ? vec[first * 3 + i] : T(0);
     }
-    out[e] = low;
+    double length[4];
+    int low[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double x = v[j * 3], y = v[j * 3 + 1], z = v[j * 3 + 2];
+      length[j] = __dadd_rn(__dadd_rn(__dmul_rn(x, x), __dmul_rn(y, y)), __dmul_rn(z, z));
+    }
+    for (int half = steps >> 1; half; half >>= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int next = low[j] + half;
+        const double border = shared ? squares[next - 1] : next <= count ? square(next - 1) : __longlong_as_double(-1);
+        low[j] = border <= length[j] ? next : low[j];
+      }
+    if (aligned && first + 4 <= edges) {
+      *reinterpret_cast<int4*>(out + first) = make_int4(low[0], low[1], low[2], low[3]);
+    } else {
+      for (int j = 0; j < 4 && first + j < edges; ++j) out[first + j] = low[j];
+    }
   }
 }
 
@@ -74,14 +99,15 @@ extern "C" int luna_distance_buckets(int dtype, const void* vec, const void* bou
   if (!status) status = bias::check_pointer(size, boundaries, "boundaries", num_boundaries > 0);
   if (!status) status = bias::check_pointer(4, out, "out", n > 0);
   if (status || n == 0) return status;
-  const int64_t ctas = ceil_div(n, 256), most = static_cast<int64_t>(rows::processors()) * 16;
+  const int64_t ctas = ceil_div(n, 1024), most = static_cast<int64_t>(rows::processors()) * 16;
+  const bool aligned = aligned_to(vec, 16) && aligned_to(out, 16);
   const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
   const int count = static_cast<int>(num_boundaries);
   const auto s = static_cast<cudaStream_t>(stream);
   if (dtype == LUNA_F64)
-    bias::buckets_kernel<double><<<grid, 256, 0, s>>>(static_cast<const double*>(vec), static_cast<const double*>(boundaries), count, out, n);
+    bias::buckets_kernel<double><<<grid, 256, 0, s>>>(static_cast<const double*>(vec), static_cast<const double*>(boundaries), count, out, n, aligned);
   else
-    bias::buckets_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(vec), static_cast<const float*>(boundaries), count, out, n);
+    bias::buckets_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(vec), static_cast<const float*>(boundaries), count, out, n, aligned);
   LUNA_LAUNCH_CHECK("distance buckets");
   return LUNA_OK;
 }

@@ -30,87 +30,139 @@ gather_kernel(const T* __restrict__ table, const int32_t* __restrict__ buckets, 
 
 // ---- gradient of the table ------------------------------------------------------------------------------------------------------
 // A CTA holds several copies of its part of the table in shared memory.  The `lanes` threads of a copy take every copies-th
-// edge of the CTA's and add its row to the copy, each thread to columns of its own: no two threads add to one number, so
-// there are no atomics, and the order of the sums depends on the sizes alone.  The copies are summed at the end, the CTAs'
-// sums in a second launch.  What bounds it is HBM where the copies are many; the additions to one copy follow one another.
+// run of AHEAD edges of the CTA's and add their rows to the copy, each thread to columns of its own: no two threads add to one
+// number, so there are no atomics, and the order of the sums depends on the sizes alone.  The copies are summed at the end,
+// the CTAs' sums in a second launch.
+//
+// Large tables leave room for few copies, so few warps, and what counts is how long an addition takes one of them: a run is
+// under way while the one before is added, its addresses are one base and its buckets one or a few wide loads, and two edges
+// are added at a time: their sums are read together, and the second takes over the first's where both are of one bucket.
+// (Four edges at a time and nothing under way: 2.6 M edges of 16 heads and 128 buckets 171 us.)
 struct Cut {
   int lanes, copies, threads;  // threads per copy; copies and threads of a CTA
-  int buckets;                 // rows of the table that a CTA has
+  int buckets;                 // rows of the table that a CTA has; each copy has one more, for what belongs to none
   int parts_of_edges, parts_of_heads, parts_of_buckets;
   int64_t shared;              // bytes
 };
 
-template <typename T, int VEC>
+template <typename T, int VEC, int AHEAD>
 __global__ void __launch_bounds__(256)
 table_kernel(const T* __restrict__ g, const int32_t* __restrict__ buckets, Acc<T>* __restrict__ partial, int64_t edges,
-             int num_buckets, int heads, Cut cut) {
+             int num_buckets, int heads, Cut cut, bool wide_buckets) {
   using A = Acc<T>;
   extern __shared__ __align__(16) unsigned char raw[];
   A* tables = reinterpret_cast<A*>(raw);
-  const int width = cut.lanes * VEC, copy_size = cut.buckets * width;
-  for (int i = threadIdx.x; i < cut.copies * copy_size; i += blockDim.x) tables[i] = A(0);
-  __syncthreads();
+  const int width = cut.lanes * VEC, copy_size = (cut.buckets + 1) * width;
   const int first_bucket = blockIdx.z * cut.buckets, first_head = blockIdx.y * width;
+  const int last_bucket = num_buckets - first_bucket < cut.buckets ? num_buckets - first_bucket : cut.buckets;
   const int lane = threadIdx.x & (cut.lanes - 1), copy = threadIdx.x / cut.lanes;
   const int head = first_head + lane * VEC;
-  const int64_t begin = edges * blockIdx.x / gridDim.x, end = edges * (blockIdx.x + 1) / gridDim.x;
-  if (copy < cut.copies && head < heads) {
-    A* mine = tables + static_cast<int64_t>(copy) * copy_size + lane * VEC;
-    constexpr int kAhead = 4;
-    for (int64_t e = begin + copy; e < end; e += static_cast<int64_t>(cut.copies) * kAhead) {
-      A v[kAhead][VEC];
-      int b[kAhead];
+  const int64_t runs = (edges + AHEAD - 1) / AHEAD, first_run = runs * blockIdx.x / gridDim.x, last_run = runs * (blockIdx.x + 1) / gridDim.x;
+  const bool works = copy < cut.copies && head < heads;
+  // this copy's runs, and the edges behind the beginning of its next one
+  const int count = works && last_run - first_run > copy ? static_cast<int>((last_run - first_run - copy + cut.copies - 1) / cut.copies) : 0;
+  int64_t at = (first_run + copy) * AHEAD;
+  const int32_t* bucket_at = buckets + at;
+  const T* g_at = g + at * heads + head;
+  const int run_step = cut.copies * AHEAD;
+  const int64_t g_step = static_cast<int64_t>(run_step) * heads;
+  using In = rows::Pack<T, VEC>;
+  using Sum = rows::Pack<A, VEC>;
+  struct Run {
+    In v[AHEAD];
+    int row[AHEAD];
+  };
+  auto fetch = [&](Run& to, int number) {
+    if (number < count && at + AHEAD <= edges) {
+      if (wide_buckets) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int64_t at = e + static_cast<int64_t>(j) * cut.copies;
-        b[j] = -1;
-        if (at < end) {
-          b[j] = buckets[at];
-          rows::load<T, VEC>(g + at * heads + head, v[j]);
-        }
+        for (int j = 0; j < AHEAD; j += 4) *reinterpret_cast<int4*>(&to.row[j]) = *reinterpret_cast<const int4*>(bucket_at + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) to.row[j] = bucket_at[j];
       }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int row = b[j] - first_bucket;
-        if (b[j] >= 0 && b[j] < num_buckets && row >= 0 && row < cut.buckets) {
-          auto* to = reinterpret_cast<rows::Pack<A, VEC>*>(mine + row * width);
-          rows::Pack<A, VEC> sum = *to;
+      for (int j = 0; j < AHEAD; ++j) to.v[j] = *reinterpret_cast<const In*>(g_at + j * heads);
+    } else {  // the last run of all may be shorter
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) sum.a[c] += v[j][c];
-          *to = sum;
+      for (int j = 0; j < AHEAD; ++j) {
+        to.row[j] = -1;
+        if (number < count && at + j < edges) {
+          to.row[j] = bucket_at[j];
+          to.v[j] = *reinterpret_cast<const In*>(g_at + j * heads);
         }
       }
     }
+    at += run_step;
+    bucket_at += run_step;
+    g_at += g_step;
+  };
+  A* mine = tables + copy * copy_size + lane * VEC;
+  auto place = [&](int row) {  // a row of another part, or none at all, goes to the row behind the last
+    return static_cast<int>(min(static_cast<unsigned>(row) - static_cast<unsigned>(first_bucket), static_cast<unsigned>(last_bucket))) * width;
+  };
+  auto add = [&](const Run& from) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; j += 2) {
+      const int p = place(from.row[j]), q = place(from.row[j + 1]);
+      Sum s = *reinterpret_cast<const Sum*>(mine + p), t = *reinterpret_cast<const Sum*>(mine + q);
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        s.a[c] += rows::widen(from.v[j].a[c]);
+        t.a[c] = (p == q ? s.a[c] : t.a[c]) + rows::widen(from.v[j + 1].a[c]);
+      }
+      *reinterpret_cast<Sum*>(mine + p) = s;
+      *reinterpret_cast<Sum*>(mine + q) = t;
+    }
+  };
+  Run one, other;
+  fetch(one, 0);
+  {
+    const Sum zeros{};
+    for (int i = threadIdx.x * VEC; i < cut.copies * copy_size; i += blockDim.x * VEC) *reinterpret_cast<Sum*>(tables + i) = zeros;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < copy_size; i += blockDim.x) {
+  for (int i = 0; i < count; i += 2) {
+    fetch(other, i + 1);
+    add(one);
+    if (i + 1 >= count) break;
+    fetch(one, i + 2);
+    add(other);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x * VEC; i < last_bucket * width; i += blockDim.x * VEC) {
     const int bucket = first_bucket + i / width, h = first_head + i % width;
-    if (bucket >= num_buckets || h >= heads) continue;
-    A sum = tables[i];
-    for (int c = 1; c < cut.copies; ++c) sum += tables[c * copy_size + i];
-    partial[(static_cast<int64_t>(blockIdx.x) * num_buckets + bucket) * heads + h] = sum;
+    if (h >= heads) continue;  // whole packets: VEC divides the heads
+    Sum sum = *reinterpret_cast<const Sum*>(tables + i);
+    for (int other_copy = 1; other_copy < cut.copies; ++other_copy) {
+      const Sum more = *reinterpret_cast<const Sum*>(tables + other_copy * copy_size + i);
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) sum.a[c] += more.a[c];
+    }
+    *reinterpret_cast<Sum*>(partial + (static_cast<int64_t>(blockIdx.x) * num_buckets + bucket) * heads + h) = sum;
   }
 }
 
-// The sums of all CTAs: 32 numbers of the table by one CTA, 16 threads for each.
-constexpr int kFinalSlices = 16;
+// The sums of all CTAs: 32 numbers of the table by one CTA, 32 threads for each.
+constexpr int kFinalSlices = 32;
 template <typename T>
 __global__ void __launch_bounds__(32 * kFinalSlices)
 table_final_kernel(const Acc<T>* __restrict__ partial, T* __restrict__ gtable, int64_t numbers, int parts) {
   using A = Acc<T>;
-  __shared__ A tile[kFinalSlices][32];
+  __shared__ A tile[kFinalSlices][33];
   wait_for_previous();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 32;
   A sum = A(0);
-  if (at < numbers)
-    for (int j = slice; j < parts; j += kFinalSlices) sum += partial[j * numbers + at];
+  if (first + lane < numbers) {
+#pragma unroll 8
+    for (int j = slice; j < parts; j += kFinalSlices) sum += partial[j * numbers + first + lane];
+  }
   tile[slice][lane] = sum;
   __syncthreads();
-  if (slice || at >= numbers) return;
-#pragma unroll
-  for (int j = 1; j < kFinalSlices; ++j) sum += tile[j][lane];
-  rows::narrow(sum, gtable[at]);
+  A total = tile[lane][slice];  // a warp's threads have the slices of one number
+  for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  if (lane == 0 && first + slice < numbers) rows::narrow(total, gtable[first + slice]);
 }
 
 // The largest packet that divides a row of `heads` and is aligned in every array.
@@ -126,31 +178,33 @@ inline int packet_of(int64_t size, int64_t heads, std::initializer_list<const vo
   return vec;
 }
 
-// How the table's gradient is cut up for packets of `vec`.  Shared memory of half a multiprocessor per CTA, or of a whole one
-// where that would leave only a few copies.
+// How the table's gradient is cut up for packets of `vec`.
 inline Cut cut_of(int64_t acc_size, int vec, int64_t edges, int64_t num_buckets, int64_t heads) {
-  constexpr int64_t kHalf = 100 * 1024, kWhole = 200 * 1024;
+  constexpr int64_t kRoom = 208 * 1024;  // of a multiprocessor's shared memory
   Cut cut{};
   const int64_t packets = ceil_div(heads, vec);
   cut.lanes = packets >= 32 ? 32 : rows::next_power_of_two(packets);
-  auto copy_bytes = [&] { return num_buckets * cut.lanes * vec * acc_size; };
-  while (cut.lanes > 1 && copy_bytes() > kWhole) cut.lanes >>= 1;
+  auto copy_bytes = [&] { return (num_buckets + 1) * cut.lanes * vec * acc_size; };
+  while (cut.lanes > 1 && copy_bytes() > kRoom) cut.lanes >>= 1;
   const int64_t row_bytes = cut.lanes * vec * acc_size;
-  cut.buckets = static_cast<int>(copy_bytes() > kWhole ? kWhole / row_bytes : num_buckets);
-  const int64_t copy = cut.buckets * row_bytes;
+  cut.buckets = static_cast<int>(copy_bytes() > kRoom ? kRoom / row_bytes - 1 : num_buckets);
+  const int64_t copy = (cut.buckets + 1) * row_bytes;
   const int64_t most = 256 / cut.lanes;
-  int64_t copies = kHalf / copy;
-  if (copies < 4) copies = kWhole / copy;
+  int64_t copies = kRoom / copy;
   copies = copies < 1 ? 1 : (copies > most ? most : copies);
+  cut.parts_of_heads = static_cast<int>(ceil_div(packets, cut.lanes));
+  cut.parts_of_buckets = static_cast<int>(ceil_div(num_buckets, cut.buckets));
+  const int64_t others = cut.parts_of_heads * static_cast<int64_t>(cut.parts_of_buckets);
+  // fewer copies where there are not eight edges (a run) for each of a GPU full of them
+  const int64_t each = ceil_div(edges, (rows::processors() > 0 ? rows::processors() : 1) * 8);
+  copies = copies < each ? copies : (each < 1 ? 1 : each);
   cut.copies = static_cast<int>(copies);
   cut.threads = static_cast<int>(ceil_div(copies * cut.lanes, 32) * 32);
   cut.shared = copies * copy;
-  cut.parts_of_heads = static_cast<int>(ceil_div(packets, cut.lanes));
-  cut.parts_of_buckets = static_cast<int>(ceil_div(num_buckets, cut.buckets));
-  const int64_t per_processor = 220 * 1024 / (cut.shared + 1024);
-  int64_t resident = rows::processors() * (per_processor < 1 ? 1 : (per_processor > 8 ? 8 : per_processor));
-  int64_t parts = resident / (cut.parts_of_heads * static_cast<int64_t>(cut.parts_of_buckets));
-  const int64_t wanted = ceil_div(edges, copies * 16);  // sixteen edges per copy at least
+  const int64_t together = kRoom / cut.shared;
+  const int64_t resident = rows::processors() * (together < 1 ? 1 : (together > 4 ? 4 : together));
+  int64_t parts = resident / others;
+  const int64_t wanted = ceil_div(edges, copies * 8);  // eight edges per copy at least
   parts = parts < wanted ? parts : wanted;
   cut.parts_of_edges = static_cast<int>(parts < 1 ? 1 : parts);
   return cut;
@@ -173,10 +227,13 @@ int table_gradient(const T* g, const int32_t* buckets, T* gtable, void* scratch,
   if (cut.parts_of_heads > 65535 || cut.parts_of_buckets > 65535)
     return fail(LUNA_ERR_UNSUPPORTED, "gradient of a table of %lld buckets and %lld heads", static_cast<long long>(num_buckets),
                 static_cast<long long>(heads));
-  LUNA_CUDA_CHECK(cudaFuncSetAttribute(table_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
   A* partial = static_cast<A*>(scratch);
-  table_kernel<T, VEC><<<dim3(cut.parts_of_edges, cut.parts_of_heads, cut.parts_of_buckets), cut.threads, cut.shared, stream>>>(
-      g, buckets, partial, edges, static_cast<int>(num_buckets), static_cast<int>(heads), cut);
+  // more edges under way where a multiprocessor has few threads
+  constexpr int kMany = VEC * sizeof(A) > 16 ? 8 : 16;  // packets of eight: the registers of eight edges are all
+  const auto kernel = cut.threads > 128 ? table_kernel<T, VEC, 8> : table_kernel<T, VEC, kMany>;
+  if (cut.shared > 40 * 1024) LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cut.shared)));
+  kernel<<<dim3(cut.parts_of_edges, cut.parts_of_heads, cut.parts_of_buckets), cut.threads, cut.shared, stream>>>(
+      g, buckets, partial, edges, static_cast<int>(num_buckets), static_cast<int>(heads), cut, aligned_to(buckets, 16));
   LUNA_LAUNCH_CHECK("gradient of the bias table");
   const int64_t numbers = num_buckets * heads;
   launch_early(table_final_kernel<T>, dim3(static_cast<unsigned>(ceil_div(numbers, 32))), 32 * kFinalSlices, 0, stream,
