@@ -53,7 +53,7 @@ struct Pair {
 };
 
 // Sums or maxima over the threads that hold the same heads of one row.
-template <typename A, int VEC>
+template <typename A, int VEC, int LANES>
 struct Together {
   const Shape& S;
   A* exchange;  // [2][warps][32][VEC]
@@ -62,6 +62,14 @@ struct Together {
 
   template <typename F>
   __device__ __forceinline__ void all(A (&v)[VEC], F&& join) {
+    if constexpr (LANES) {
+#pragma unroll
+      for (int off = LANES >> 1; off; off >>= 1)
+        if (off >= S.across)
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) v[c] = join(v[c], __shfl_xor_sync(0xffffffffu, v[c], off));
+      return;
+    }
     const int within = S.lanes < 32 ? S.lanes : 32;
     for (int off = within >> 1; off >= S.across; off >>= 1)
 #pragma unroll
@@ -91,82 +99,104 @@ struct Together {
   }
 };
 
-__device__ __forceinline__ float exponential(float v) { return expf(v); }
-__device__ __forceinline__ double exponential(double v) { return exp(v); }
+// exp(z - m), in single precision as 2^((z - m) log2 e): a product, rounded once, and an instruction that is off by two units in
+// the last place.  The difference is made first: z and m may be the lowest numbers of their type.
+__device__ __forceinline__ float exponential(float z, float m) {
+  float v;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"((z - m) * 1.4426950408889634f));
+  return v;
+}
+__device__ __forceinline__ double exponential(double z, double m) { return exp(z - m); }
+// Of a sum of exponentials: at least one (the largest logit's), or zero, or no number.
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return v == 0.0f ? 0.0f : r;
+}
+__device__ __forceinline__ double reciprocal(double v) { return v == 0.0 ? 0.0 : 1.0 / v; }
 
 template <typename A>
 __device__ __forceinline__ A lowest() {
   return -static_cast<A>(INFINITY);
 }
+// What is taken out of the logits: the largest one, or nothing where there is none (nothing left, or nothing but NaN).
+template <typename A>
+__device__ __forceinline__ A taken(A largest) {
+  return largest == lowest<A>() ? A(0) : largest;
+}
 
-template <typename T, int VEC, int K, int ORDER, int PHASE>
+// LANES: as S.lanes, where an edge's heads fill their `across` packets, so that a row is one stretch of packets; 0: neither is known.
+template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES>
 __global__ void __launch_bounds__(kThreads, ORDER == kSecond ? 2 : ORDER == kForward ? 3 : 4)
 rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __restrict__ stats) {
   using A = Acc<T>;
+  using In = rows::Pack<T, VEC>;
   __shared__ A exchange[2 * kThreads * VEC];
-  Together<A, VEC> together(S, exchange);
-  const int lane = threadIdx.x & (S.lanes - 1);
-  const int slot = lane / S.across, slots = S.lanes / S.across;
+  Together<A, VEC, LANES> together(S, exchange);
+  const int lanes = LANES ? LANES : S.lanes;
+  const int lane = threadIdx.x & (lanes - 1);
+  const int slot = lane / S.across, slots = lanes / S.across;
   const int head = (blockIdx.y * S.across + (lane & (S.across - 1))) * VEC;
-  const bool here = head < S.heads;
-  const int teams = kThreads / S.lanes, team = threadIdx.x / S.lanes;
-  const int ahead = S.lanes < 32 ? team % (32 / S.lanes) : 0;  // teams of this warp before this one: they leave together
+  const bool here = LANES || head < S.heads;
+  const int teams = kThreads / lanes, team = threadIdx.x / lanes;
+  const int ahead = lanes < 32 ? team % (32 / lanes) : 0;  // teams of this warp before this one: they leave together
+  const int stride = LANES ? LANES * VEC : slots * S.heads;  // from one of a thread's edges to the next
 
   // K edges of a thread: z (forward), or alpha and g and the cotangent r
   A u[K][VEC], g[K][VEC], r[K][VEC];
   const T* const table = ORDER == kForward ? o.table : ORDER == kSecond ? o.rtable : nullptr;
-  const int stride = slots * S.heads;
-  using In = rows::Pack<T, VEC>;
-  auto fetch = [&](int64_t first, int64_t end) {
-    In t[K];
-    int bucket[K];
-    bool keep[K];
-    const int left = end - first > K * slots ? K * slots : static_cast<int>(end - first);  // this thread's edges: k * slots < left
-    const int64_t at = first * S.heads + head;
+  // `first`: the thread's first edge of the batch; `left`: edges of the row from there on
+  auto fetch = [&](int first, int left) {
+    const int64_t at = static_cast<int64_t>(first) * S.heads + head;
     auto there = [&](int k) { return k * slots < left; };
     auto bring = [&](const T* __restrict__ array, A (&to)[K][VEC], A otherwise) {
+      const T* from = array + at;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (there(k)) {
-          rows::load<T, VEC>(array + at + k * stride, to[k]);
+          rows::load<T, VEC>(from + k * stride, to[k]);
         } else {
 #pragma unroll
           for (int c = 0; c < VEC; ++c) to[k][c] = otherwise;
         }
       }
     };
-    auto nothing = [&](A (&to)[K][VEC]) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) to[k][c] = A(0);
-    };
+    int bucket[K];
+    bool keep[K];
     if (table) {
+      const int32_t* from = o.buckets + first;
 #pragma unroll
-      for (int k = 0; k < K; ++k) bucket[k] = there(k) ? o.buckets[first + k * slots] : -1;
+      for (int k = 0; k < K; ++k) bucket[k] = there(k) ? from[k * slots] : -1;
     }
     if constexpr (ORDER == kForward) {
       if (o.mask) {
+        const uint8_t* from = o.mask + first;
 #pragma unroll
-        for (int k = 0; k < K; ++k) keep[k] = there(k) && o.mask[first + k * slots];
+        for (int k = 0; k < K; ++k) keep[k] = there(k) && from[k * slots];
       }
       bring(o.logits, u, lowest<A>());
     } else {
       bring(o.alpha, u, A(0));
       bring(o.g, g, A(0));
       if constexpr (ORDER == kSecond) {
-        if (o.r)
+        if (o.r) {
           bring(o.r, r, A(0));
-        else
-          nothing(r);
+        } else {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) r[k][c] = A(0);
+        }
       }
     }
     if (table) {
+      const T* const from = table + head;
+      In t[K];
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) t[k].a[c] = T(0);
-        if (bucket[k] >= 0 && bucket[k] < S.num_buckets) t[k] = *reinterpret_cast<const In*>(table + static_cast<int64_t>(bucket[k]) * S.heads + head);
+        t[k] = In{};
+        if (static_cast<unsigned>(bucket[k]) < static_cast<unsigned>(S.num_buckets))
+          t[k] = *reinterpret_cast<const In*>(from + static_cast<int64_t>(bucket[k]) * S.heads);
       }
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -182,44 +212,102 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
       }
     }
   };
+  // The outputs of a batch, from alpha times `factor` (forward), or from alpha, D and R
+  auto put = [&](int first, int left, const A (&a)[VEC], const A (&b)[VEC]) {
+    const int64_t at = static_cast<int64_t>(first) * S.heads + head;
+    T *const out = o.out + at, *const out2 = o.out2 + at;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k * slots >= left) continue;
+      A v[VEC], w[VEC];
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        const A alpha = u[k][c];
+        if constexpr (ORDER == kForward) {
+          v[c] = alpha * b[c];
+        } else if constexpr (ORDER == kBackward) {
+          v[c] = alpha != A(0) ? alpha * (g[k][c] - a[c]) : A(0);
+        } else {
+          v[c] = alpha != A(0) ? alpha * (r[k][c] - b[c]) : A(0);
+          w[c] = alpha != A(0) ? r[k][c] * (g[k][c] - a[c]) - g[k][c] * b[c] : A(0);
+        }
+      }
+      if (ORDER != kSecond || o.out) rows::store<T, VEC>(out + k * stride, v);
+      if constexpr (ORDER == kSecond)
+        if (o.out2) rows::store<T, VEC>(out2 + k * stride, w);
+    }
+  };
+  auto exponentials = [&](const A (&m)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) u[k][c] = exponential(u[k][c], m[c]);
+  };
+  auto largest = [&](A (&a)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) a[c] = fmax(a[c], u[k][c]);
+  };
+  auto add_up = [&](A (&b)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) b[c] += u[k][c];
+  };
 
+  const int batch = K * slots;
   const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team; row - ahead < R.count; row += step) {
-    int64_t begin = 0, end = 0;
+    int first = 0, length = 0;
     if (row < R.count && here) {
-      begin = R.rowptr[row];
-      end = R.rowptr[row + 1];
+      first = R.rowptr[row];
+      length = R.rowptr[row + 1] - first;
     }
-    const int64_t batch = static_cast<int64_t>(K) * slots;
-    const int64_t last = begin + slot + (end > begin ? (end - begin - 1) / batch * batch : 0);  // the thread's place in the last batch
-    begin += slot;
+    first += slot;
+    const int left = length - slot;
+    const int behind = length > 0 ? (length - 1) / batch * batch : 0;  // where the last batch begins
     A a[VEC], b[VEC];  // forward: the largest logit and the sum; else D and R
 #pragma unroll
     for (int c = 0; c < VEC; ++c) {
       a[c] = ORDER == kForward ? lowest<A>() : A(0);
       b[c] = A(0);
     }
-    A factor[VEC];  // forward: from the exponentials in registers to alpha
     if constexpr (PHASE != kApply) {
-      // From the last batch to the first, which stays in registers.  Forward: each thread has a largest logit and a sum of its
-      // own, which grow together, and keeps exp(z - its largest).
-      for (int64_t e = last; e >= begin; e -= batch) {
-        fetch(e, end);
-        if constexpr (ORDER == kForward) {
+      if constexpr (ORDER == kForward) {
+        // Batches behind the first one: each thread has a largest logit and a sum of its own, which grow together.
+        for (int at = behind; at > 0; at -= batch) {
+          fetch(first + at, left - at);
+          A before[VEC], m[VEC];
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) before[c] = a[c];
+          largest(a);
 #pragma unroll
           for (int c = 0; c < VEC; ++c) {
-            const A before = a[c];
-#pragma unroll
-            for (int k = 0; k < K; ++k) a[c] = fmax(a[c], u[k][c]);
-            const A shift = a[c] == lowest<A>() ? A(0) : a[c];  // nothing left, or nothing but NaN
-            if (b[c] != A(0)) b[c] *= exponential((before == lowest<A>() ? shift : before) - shift);
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-              u[k][c] = exponential(u[k][c] - shift);
-              b[c] += u[k][c];
-            }
+            m[c] = taken(a[c]);
+            if (b[c] != A(0)) b[c] *= before[c] == lowest<A>() ? A(1) : exponential(before[c], m[c]);
           }
-        } else {
+          exponentials(m);
+          add_up(b);
+        }
+        A own[VEC], m[VEC];
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) own[c] = a[c];
+        fetch(first, left);
+        largest(a);
+        together.max(a);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          m[c] = taken(a[c]);
+          if (b[c] != A(0)) b[c] *= own[c] == lowest<A>() ? A(1) : exponential(own[c], m[c]);
+        }
+        exponentials(m);
+        add_up(b);
+        together.sum(b);
+      } else {
+        // From the last batch to the first, which stays in registers
+        for (int at = behind; at >= 0; at -= batch) {
+          fetch(first + at, left - at);
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -228,20 +316,6 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
               if constexpr (ORDER == kSecond) b[c] += u[k][c] != A(0) ? u[k][c] * r[k][c] : A(0);
             }
         }
-      }
-      if constexpr (ORDER == kForward) {
-        A own[VEC];
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) own[c] = a[c];
-        together.max(a);
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) {
-          const A shift = a[c] == lowest<A>() ? A(0) : a[c];
-          factor[c] = own[c] == lowest<A>() ? A(1) : exponential(own[c] - shift);
-          b[c] *= factor[c];
-        }
-        together.sum(b);
-      } else {
         together.sum(a);
         if constexpr (ORDER == kSecond) together.sum(b);
       }
@@ -265,44 +339,15 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
       if constexpr (ORDER == kForward) {
 #pragma unroll
         for (int c = 0; c < VEC; ++c) {
-          a[c] = a[c] == lowest<A>() ? A(0) : a[c];
-          b[c] = b[c] == A(0) ? A(0) : A(1) / b[c];
-          if constexpr (PHASE == kWhole) factor[c] *= b[c];
+          a[c] = taken(a[c]);
+          b[c] = reciprocal(b[c]);
         }
       }
-      for (int64_t e = begin; e <= last; e += batch) {
-        if (PHASE == kApply || e > begin) {
-          fetch(e, end);
-          if constexpr (ORDER == kForward) {
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) {
-              factor[c] = b[c];
-#pragma unroll
-              for (int k = 0; k < K; ++k) u[k][c] = exponential(u[k][c] - a[c]);
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (e + k * slots >= end) continue;
-          const int64_t at = e * S.heads + head + k * stride;
-          A v[VEC], w[VEC];
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) {
-            const A alpha = u[k][c];
-            if constexpr (ORDER == kForward) {
-              v[c] = alpha * factor[c];
-            } else if constexpr (ORDER == kBackward) {
-              v[c] = alpha != A(0) ? alpha * (g[k][c] - a[c]) : A(0);
-            } else {
-              v[c] = alpha != A(0) ? alpha * (r[k][c] - b[c]) : A(0);
-              w[c] = alpha != A(0) ? r[k][c] * (g[k][c] - a[c]) - g[k][c] * b[c] : A(0);
-            }
-          }
-          if (o.out) rows::store<T, VEC>(o.out + at, v);
-          if constexpr (ORDER == kSecond)
-            if (o.out2) rows::store<T, VEC>(o.out2 + at, w);
-        }
+      if constexpr (PHASE == kWhole) put(first, left, a, b);
+      for (int at = PHASE == kWhole ? batch : 0; at <= behind; at += batch) {
+        fetch(first + at, left - at);
+        if constexpr (ORDER == kForward) exponentials(a);
+        put(first + at, left - at, a, b);
       }
     }
   }
@@ -321,8 +366,8 @@ join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
   // one pair after the other; a pair without a largest logit has nothing (a sum of zero), or nothing but NaN, in its sum too
   auto join = [](Pair<A> p, Pair<A> q) {
     if (!FORWARD) return Pair<A>{p.a + q.a, p.b + q.b};
-    const A top = fmax(p.a, q.a), shift = top == lowest<A>() ? A(0) : top;
-    return Pair<A>{top, (p.a == lowest<A>() ? p.b : p.b * exponential(p.a - shift)) + (q.a == lowest<A>() ? q.b : q.b * exponential(q.a - shift))};
+    const A top = fmax(p.a, q.a), m = taken(top);
+    return Pair<A>{top, (p.a == lowest<A>() ? p.b : p.b * exponential(p.a, m)) + (q.a == lowest<A>() ? q.b : q.b * exponential(q.a, m))};
   };
   for (int base = 0; base < heads; base += across) {
     const int h = base + (lane & (across - 1));
@@ -336,11 +381,11 @@ join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
   }
 }
 
-template <typename T, int VEC, int K, int ORDER, int PHASE>
+template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES = 0>
 int start(const Rows& R, const Shape& S, const Operands<T>& o, Pair<Acc<T>>* stats, cudaStream_t stream) {
   const int64_t ctas = ceil_div(R.count, kThreads / S.lanes), most = static_cast<int64_t>(rows::processors()) * 256;
   const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most), static_cast<unsigned>(ceil_div(S.heads, S.across * VEC)));
-  rows_kernel<T, VEC, K, ORDER, PHASE><<<grid, kThreads, 0, stream>>>(R, S, o, stats);
+  rows_kernel<T, VEC, K, ORDER, PHASE, LANES><<<grid, kThreads, 0, stream>>>(R, S, o, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges");
   return LUNA_OK;
 }
@@ -358,7 +403,11 @@ int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, con
   const int64_t wanted = ceil_div(mean + mean / 4, K) * S.across;
   S.lanes = wanted > 128 ? kThreads : wanted >= 32 ? 32 : rows::next_power_of_two(wanted);
   auto* stats = static_cast<Pair<Acc<T>>*>(scratch);
-  if (!R.first) return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
+  if (!R.first) {
+    if (S.across * VEC == S.heads && S.lanes == 32) return start<T, VEC, K, ORDER, kWhole, 32>(R, S, o, stats, stream);
+    if (S.across * VEC == S.heads && S.lanes == 16) return start<T, VEC, K, ORDER, kWhole, 16>(R, S, o, stats, stream);
+    return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
+  }
   if (const int status = start<T, VEC, K, ORDER, kSums>(R, S, o, stats, stream)) return status;
   join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(ceil_div(R.nodes, kThreads / 32)), kThreads, 0, stream>>>(R, S.heads, S.across, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges: pieces");

@@ -73,6 +73,13 @@ table_kernel(const T* __restrict__ g, const int32_t* __restrict__ buckets, Acc<T
     int row[AHEAD];
   };
   auto fetch = [&](Run& to, int number) {
+    // The run after the next one is called into L2: registers hold one run under way, which does not cover the way to memory.
+    if (number + 2 < count && at + 2 * static_cast<int64_t>(run_step) + AHEAD <= edges) {
+      const char* line = reinterpret_cast<const char*>(g_at + 2 * g_step - lane * VEC);
+      for (int i = lane * 128; i < (AHEAD * heads - first_head) * static_cast<int>(sizeof(T)); i += cut.lanes * 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(line + i));
+      if (lane == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(bucket_at + 2 * run_step));
+    }
     if (number < count && at + AHEAD <= edges) {
       if (wide_buckets) {
 #pragma unroll
