@@ -295,8 +295,10 @@ LUNA_API int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* buc
 
 /* --------------------------------------------------------------------------------------------------------------
  * Softmax over the in-edges of every node, for logits[num_edges, heads] whose edges are sorted by destination.
- * Row i is the edges rowptr[i] .. rowptr[i+1]-1.  Where a node's edges are cut into several rows (so that a long row does
- * not hold one multiprocessor), first[node] is the node's first row, node[row] the row's node; else both are null.
+ * Row i is the edges rowptr[i] .. rowptr[i+1]-1.  A node's edges are one row, unless there are so many that they would hold one
+ * multiprocessor: such a node's edges are cut into several rows, its pieces.  The num_cut nodes are numbered from zero, and
+ * so are their num_pieces pieces, node by node: those of node c are cut_first[c] .. cut_first[c+1]-1.  piece_of_row[row] is a
+ * row's piece, or -1; row_of_piece and cut_of_piece lead back.  Without cut nodes the four tables are null.
  *
  * forward:  alpha = softmax(logits + table[buckets]) over the unmasked edges of each node (mask[e] = 0: left out, alpha 0);
  *           a node without any, or with logits of -inf only, gets zeros.  table, buckets, mask may be null.
@@ -305,10 +307,12 @@ LUNA_API int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* buc
  * second:   with r, rtable the cotangents of glogits, gtable (null: zero), the derivatives with respect to alpha and g;
  *           null outputs are skipped. */
 typedef struct {
-  int64_t num_rows, num_edges, num_nodes;
+  int64_t num_rows, num_edges, num_pieces, num_cut;
   const int32_t* rowptr;
-  const int64_t* first;
-  const int64_t* node;
+  const int32_t* piece_of_row;
+  const int32_t* row_of_piece;
+  const int32_t* cut_of_piece;
+  const int32_t* cut_first;
 } luna_row_table;
 /* num_buckets: 0 for calls without a gradient of a table. */
 LUNA_API int64_t luna_graph_softmax_scratch_bytes(int dtype, const luna_row_table* rows, int64_t heads, int64_t num_buckets);

@@ -93,8 +93,8 @@ class NormDesc(ctypes.Structure):
 
 
 class RowTable(ctypes.Structure):
-    _fields_ = [("num_rows", ctypes.c_int64), ("num_edges", ctypes.c_int64), ("num_nodes", ctypes.c_int64),
-                ("rowptr", ctypes.c_void_p), ("first", ctypes.c_void_p), ("node", ctypes.c_void_p)]
+    _fields_ = [(name, ctypes.c_int64) for name in ("num_rows", "num_edges", "num_pieces", "num_cut")] + [
+        (name, ctypes.c_void_p) for name in ("rowptr", "piece_of_row", "row_of_piece", "cut_of_piece", "cut_first")]
 
 
 # name -> (restype, argtypes); mirrors include/luna_b200.h

@@ -16,14 +16,19 @@ int describe(const Call& c, Rows* R) {
   if (c.dtype < LUNA_F32 || c.dtype > LUNA_F16) return fail(LUNA_ERR_INVALID_ARGUMENT, "unknown dtype %d", c.dtype);
   if (!c.table) return fail(LUNA_ERR_INVALID_ARGUMENT, "null row table");
   const luna_row_table& t = *c.table;
-  if (t.num_rows < 0 || t.num_edges < 0 || t.num_nodes < 0 || c.num_buckets < 0) return fail(LUNA_ERR_INVALID_ARGUMENT, "negative size");
+  if (t.num_rows < 0 || t.num_edges < 0 || t.num_pieces < 0 || t.num_cut < 0 || c.num_buckets < 0)
+    return fail(LUNA_ERR_INVALID_ARGUMENT, "negative size");
   if (c.heads < 1) return fail(LUNA_ERR_INVALID_ARGUMENT, "softmax needs a head at least");
   if (c.heads >= (1 << 20)) return fail(LUNA_ERR_UNSUPPORTED, "softmax of %lld heads", static_cast<long long>(c.heads));
   if (c.num_buckets >= (1 << 30)) return fail(LUNA_ERR_UNSUPPORTED, "softmax with %lld buckets", static_cast<long long>(c.num_buckets));
-  if (t.num_rows >= (1ll << 31) || t.num_edges >= (1ll << 31)) return fail(LUNA_ERR_OVERFLOW, "graph exceeds the 32-bit index range of this build");
+  if (t.num_rows >= (1ll << 31) || t.num_edges >= (1ll << 31) - 1024)
+    return fail(LUNA_ERR_OVERFLOW, "graph exceeds the 32-bit index range of this build");
   if (t.num_edges > 0 && (t.num_rows == 0 || !t.rowptr)) return fail(LUNA_ERR_INVALID_ARGUMENT, "row pointers missing");
-  if (!t.first != !t.node) return fail(LUNA_ERR_INVALID_ARGUMENT, "pieces of rows need both of their tables");
-  *R = Rows{t.rowptr, t.num_rows, t.first, t.node, t.num_nodes};
+  if (t.num_pieces > t.num_rows || t.num_cut > t.num_pieces || (t.num_pieces > 0) != (t.num_cut > 0))
+    return fail(LUNA_ERR_INVALID_ARGUMENT, "pieces that no rows have");
+  if (t.num_pieces > 0 && (!t.piece_of_row || !t.row_of_piece || !t.cut_of_piece || !t.cut_first))
+    return fail(LUNA_ERR_INVALID_ARGUMENT, "tables of the pieces missing");
+  *R = Rows{t.rowptr, t.num_rows, t.num_pieces, t.num_cut, t.piece_of_row, t.row_of_piece, t.cut_of_piece, t.cut_first};
   return LUNA_OK;
 }
 
@@ -34,8 +39,7 @@ int pointer(const Call& c, const void* p, const char* name, bool required) {
 
 // Room for the sums of the pieces, rounded up, so that what follows it is aligned.
 int64_t pieces_bytes(const Call& c) {
-  if (!c.table->first) return 0;
-  return ceil_div(c.table->num_rows * c.heads * 2 * rows::acc_size_of(c.dtype), 16) * 16;
+  return ceil_div(c.table->num_pieces * c.heads * 2 * rows::acc_size_of(c.dtype), 16) * 16;
 }
 
 int scratch_fits(int64_t needed, const void* scratch, int64_t bytes) {

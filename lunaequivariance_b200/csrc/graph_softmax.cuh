@@ -10,8 +10,8 @@
 // of a thread); the rest of a longer row passes twice, the second time from cache.  All loads of a batch are under way before
 // the first is waited for: with the mask and the table looked up edge by edge, 2.6 M edges with 8 heads took 94 us forward.
 // `lanes` threads of a warp share a row, or a whole CTA where rows are long; of them `across` (a power of two) lie side by side
-// over an edge's heads.  Rows of more than a thousand edges come cut into pieces: one launch makes the pieces' sums, one joins
-// those of each node, and one makes the outputs.
+// over an edge's heads.  Very long rows come cut into pieces: the first launch makes the outputs of whole rows and the sums of
+// pieces, one joins those of each cut node, and one makes the pieces' outputs.
 #pragma once
 
 #include "rows.cuh"
@@ -23,12 +23,10 @@ using rows::Acc;
 
 constexpr int kThreads = 256;
 
-struct Rows {
+struct Rows {  // as luna_row_table
   const int32_t* rowptr;
-  int64_t count;
-  const int64_t* first;  // of a node's pieces; null where rows are not cut
-  const int64_t* node;   // of a piece
-  int64_t nodes;
+  int64_t count, pieces, cut;
+  const int32_t *piece_of_row, *row_of_piece, *cut_of_piece, *cut_first;
 };
 
 struct Shape {
@@ -37,7 +35,7 @@ struct Shape {
 };
 
 enum Order { kForward, kBackward, kSecond };
-enum Phase { kWhole, kSums, kApply };
+enum Phase { kWhole, kMixed, kApply };  // no pieces; whole rows and the pieces' sums; the pieces' outputs
 
 template <typename T>
 struct Operands {
@@ -127,7 +125,7 @@ __device__ __forceinline__ A taken(A largest) {
 
 // LANES: as S.lanes, where an edge's heads fill their `across` packets, so that a row is one stretch of packets; 0: neither is known.
 template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES>
-__global__ void __launch_bounds__(kThreads, ORDER == kSecond ? 2 : ORDER == kForward ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, ORDER == kBackward ? 4 : ORDER == kForward && sizeof(T) <= 4 ? 3 : 2)
 rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __restrict__ stats) {
   using A = Acc<T>;
   using In = rows::Pack<T, VEC>;
@@ -258,9 +256,12 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
 
   const int batch = K * slots;
   const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team; row - ahead < R.count; row += step) {
-    int first = 0, length = 0;
-    if (row < R.count && here) {
+  const int64_t count = PHASE == kApply ? R.pieces : R.count;
+  for (int64_t number = static_cast<int64_t>(blockIdx.x) * teams + team; number - ahead < count; number += step) {
+    int first = 0, length = 0, piece = -1;
+    if (number < count && here) {
+      const int64_t row = PHASE == kApply ? R.row_of_piece[number] : number;
+      if constexpr (PHASE == kMixed) piece = R.piece_of_row[row];
       first = R.rowptr[row];
       length = R.rowptr[row + 1] - first;
     }
@@ -320,49 +321,46 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
         if constexpr (ORDER == kSecond) together.sum(b);
       }
     }
-    if constexpr (PHASE == kSums) {
-      if (row < R.count && here && slot == 0)
+    if (PHASE == kMixed && piece >= 0) {
+      if (slot == 0)
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) stats[row * S.heads + head + c] = Pair<A>{a[c], b[c]};
-    } else {
-      if constexpr (PHASE == kApply) {
-        if (row < R.count && here) {
-          const int64_t at = R.first[R.node[row]] * S.heads + head;
-#pragma unroll
-          for (int c = 0; c < VEC; ++c) {
-            const Pair<A> known = stats[at + c];
-            a[c] = known.a;
-            b[c] = known.b;
-          }
-        }
-      }
-      if constexpr (ORDER == kForward) {
+        for (int c = 0; c < VEC; ++c) stats[static_cast<int64_t>(piece) * S.heads + head + c] = Pair<A>{a[c], b[c]};
+      continue;
+    }
+    if constexpr (PHASE == kApply) {
+      if (number < count && here) {
+        const int64_t at = static_cast<int64_t>(R.cut_first[R.cut_of_piece[number]]) * S.heads + head;
 #pragma unroll
         for (int c = 0; c < VEC; ++c) {
-          a[c] = taken(a[c]);
-          b[c] = reciprocal(b[c]);
+          const Pair<A> known = stats[at + c];
+          a[c] = known.a;
+          b[c] = known.b;
         }
       }
-      if constexpr (PHASE == kWhole) put(first, left, a, b);
-      for (int at = PHASE == kWhole ? batch : 0; at <= behind; at += batch) {
-        fetch(first + at, left - at);
-        if constexpr (ORDER == kForward) exponentials(a);
-        put(first + at, left - at, a, b);
+    }
+    if constexpr (ORDER == kForward) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        a[c] = taken(a[c]);
+        b[c] = reciprocal(b[c]);
       }
+    }
+    if constexpr (PHASE != kApply) put(first, left, a, b);
+    for (int at = PHASE != kApply ? batch : 0; at <= behind; at += batch) {
+      fetch(first + at, left - at);
+      if constexpr (ORDER == kForward) exponentials(a);
+      put(first + at, left - at, a, b);
     }
   }
 }
 
-// Joins the sums of the pieces of every node that has several, in its first piece's place: a warp per node, `across` of its
-// threads (a power of two) side by side over the heads.
+// Joins the sums of the pieces of every cut node, in its first piece's place: a CTA per node, `across` of its threads (a power
+// of two, at most a warp) side by side over the heads.
 template <typename A, bool FORWARD>
 __global__ void __launch_bounds__(kThreads)
 join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
-  const int lane = threadIdx.x & 31;
-  const int64_t node = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  if (node >= R.nodes) return;
-  const int64_t first = R.first[node], pieces = (node + 1 < R.nodes ? R.first[node + 1] : R.count) - first;
-  if (pieces < 2) return;
+  __shared__ Pair<A> tile[kThreads];
+  const int64_t first = R.cut_first[blockIdx.x], pieces = R.cut_first[blockIdx.x + 1] - first;
   // one pair after the other; a pair without a largest logit has nothing (a sum of zero), or nothing but NaN, in its sum too
   auto join = [](Pair<A> p, Pair<A> q) {
     if (!FORWARD) return Pair<A>{p.a + q.a, p.b + q.b};
@@ -370,20 +368,25 @@ join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
     return Pair<A>{top, (p.a == lowest<A>() ? p.b : p.b * exponential(p.a, m)) + (q.a == lowest<A>() ? q.b : q.b * exponential(q.a, m))};
   };
   for (int base = 0; base < heads; base += across) {
-    const int h = base + (lane & (across - 1));
+    const int h = base + (threadIdx.x & (across - 1));
     Pair<A> sum{FORWARD ? lowest<A>() : A(0), A(0)};
-    if (h < heads)
-      for (int64_t p = lane / across; p < pieces; p += 32 / across) sum = join(sum, stats[(first + p) * heads + h]);
-    for (int off = 16; off >= across; off >>= 1)
-      sum = join(sum, Pair<A>{__shfl_xor_sync(0xffffffffu, sum.a, off), __shfl_xor_sync(0xffffffffu, sum.b, off)});
-    __syncwarp();  // all have read the first piece
-    if (lane < across && h < heads) stats[first * heads + h] = sum;
+    if (h < heads) {
+#pragma unroll 4
+      for (int64_t p = threadIdx.x / across; p < pieces; p += kThreads / across) sum = join(sum, stats[(first + p) * heads + h]);
+    }
+    __syncthreads();
+    tile[threadIdx.x] = sum;
+    for (int off = kThreads / 2; off >= across; off >>= 1) {
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < off) tile[threadIdx.x] = join(tile[threadIdx.x], tile[threadIdx.x + off]);
+    }
+    if (static_cast<int>(threadIdx.x) < across && h < heads) stats[first * heads + h] = tile[threadIdx.x];  // all have read the first piece
   }
 }
 
 template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES = 0>
 int start(const Rows& R, const Shape& S, const Operands<T>& o, Pair<Acc<T>>* stats, cudaStream_t stream) {
-  const int64_t ctas = ceil_div(R.count, kThreads / S.lanes), most = static_cast<int64_t>(rows::processors()) * 256;
+  const int64_t ctas = ceil_div(PHASE == kApply ? R.pieces : R.count, kThreads / S.lanes), most = static_cast<int64_t>(rows::processors()) * 256;
   const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most), static_cast<unsigned>(ceil_div(S.heads, S.across * VEC)));
   rows_kernel<T, VEC, K, ORDER, PHASE, LANES><<<grid, kThreads, 0, stream>>>(R, S, o, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges");
@@ -398,18 +401,18 @@ int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, con
   S.num_buckets = static_cast<int>(num_buckets);
   const int64_t packets = heads / VEC;
   S.across = packets >= 32 ? 32 : rows::next_power_of_two(packets);
-  // As many threads as hold a row somewhat longer than the mean; a CTA where a warp would read most of a row twice.
+  // As many threads as hold a row (of the pieces, one) somewhat longer than the mean; a CTA where a warp would read most of a row twice.
   const int64_t mean = ceil_div(edges, R.count);
   const int64_t wanted = ceil_div(mean + mean / 4, K) * S.across;
   S.lanes = wanted > 128 ? kThreads : wanted >= 32 ? 32 : rows::next_power_of_two(wanted);
   auto* stats = static_cast<Pair<Acc<T>>*>(scratch);
-  if (!R.first) {
+  if (!R.pieces) {
     if (S.across * VEC == S.heads && S.lanes == 32) return start<T, VEC, K, ORDER, kWhole, 32>(R, S, o, stats, stream);
     if (S.across * VEC == S.heads && S.lanes == 16) return start<T, VEC, K, ORDER, kWhole, 16>(R, S, o, stats, stream);
     return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
   }
-  if (const int status = start<T, VEC, K, ORDER, kSums>(R, S, o, stats, stream)) return status;
-  join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(ceil_div(R.nodes, kThreads / 32)), kThreads, 0, stream>>>(R, S.heads, S.across, stats);
+  if (const int status = start<T, VEC, K, ORDER, kMixed>(R, S, o, stats, stream)) return status;
+  join_kernel<Acc<T>, ORDER == kForward><<<static_cast<unsigned>(R.cut), kThreads, 0, stream>>>(R, S.heads, S.across, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges: pieces");
   return start<T, VEC, K, ORDER, kApply>(R, S, o, stats, stream);
 }

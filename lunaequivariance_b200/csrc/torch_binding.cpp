@@ -1047,17 +1047,21 @@ Tensor relative_bias(const Tensor& table, const Tensor& buckets) {
 
 // ---- softmax over in-edges ----------------------------------------------------------------------------------------------------------
 struct Rows : torch::CustomClassHolder {
-  std::array<Tensor, 3> tables;  // rowptr; of cut rows the first piece of each node and the node of each piece
+  std::array<Tensor, 5> tables;  // rowptr, and of the pieces of cut rows: those of the rows, their rows, their nodes, the nodes' first ones
   luna_row_table native{};
-  Rows(const Tensor& rowptr, int64_t edges, const Maybe& first, const Maybe& node) : tables{rowptr, of(first), of(node)} {
+  Rows(const Tensor& rowptr, int64_t edges, const Maybe& piece_of_row, const Maybe& row_of_piece, const Maybe& cut_of_piece,
+       const Maybe& cut_first)
+      : tables{rowptr, of(piece_of_row), of(row_of_piece), of(cut_of_piece), of(cut_first)} {
     native.num_rows = rowptr.numel() - 1;
     native.num_edges = edges;
     native.rowptr = rowptr.data_ptr<int32_t>();
-    native.num_nodes = native.num_rows;
-    if (!first) return;
-    native.num_nodes = first->numel();
-    native.first = first->data_ptr<int64_t>();
-    native.node = node->data_ptr<int64_t>();
+    if (!piece_of_row) return;
+    native.num_pieces = row_of_piece->numel();
+    native.num_cut = cut_first->numel() - 1;
+    native.piece_of_row = piece_of_row->data_ptr<int32_t>();
+    native.row_of_piece = row_of_piece->data_ptr<int32_t>();
+    native.cut_of_piece = cut_of_piece->data_ptr<int32_t>();
+    native.cut_first = cut_first->data_ptr<int32_t>();
   }
 };
 using RowsPtr = c10::intrusive_ptr<Rows>;
@@ -1228,7 +1232,7 @@ PYBIND11_MODULE(luna_torch, m) {
   m.def("conv", torch::wrap_pybind_function(conv));
   m.def("harmonics", torch::wrap_pybind_function(harmonics));
   py::class_<Norm, NormPtr>(m, "Norm").def(py::init<const std::vector<std::array<int64_t, 3>>&, int64_t, double>());
-  py::class_<Rows, RowsPtr>(m, "Rows").def(py::init<const Tensor&, int64_t, const Maybe&, const Maybe&>());
+  py::class_<Rows, RowsPtr>(m, "Rows").def(py::init<const Tensor&, int64_t, const Maybe&, const Maybe&, const Maybe&, const Maybe&>());
   m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
   m.def("distance_buckets", torch::wrap_pybind_function(distance_buckets));
   m.def("relative_bias", torch::wrap_pybind_function(relative_bias));

@@ -21,6 +21,8 @@ SOURCE_SEGMENT_EDGES = 32
 # A warp walks a node's edges one after the other, so a node with very many edges would hold one warp for the whole
 # launch.  Rows longer than this are cut into virtual rows of at most this many edges (LunaTPGraph.split_rows).
 ROW_SPLIT_EDGES = 1024
+# Operators that read a row as a whole cut long rows into pieces of this many edges (LunaTPGraph.row_holder).
+ROW_PIECE_EDGES = 256
 _TABLE_LIMIT = (1 << 31) - 1024  # entries of a table with 32-bit indices
 
 
@@ -137,17 +139,21 @@ class LunaTPGraph:
         return holder
 
     def row_holder(self):
-        """The rows of in-edges for the C++ launch path, long ones cut into pieces of ``ROW_SPLIT_EDGES`` edges."""
+        """The rows of in-edges for the C++ launch path of the operators that go through them as a whole.
+
+        A row of more than ``ROW_SPLIT_EDGES`` edges, or of half as many where that is four times the mean, would keep one
+        multiprocessor busy when all others are done: such rows are cut into pieces of ``ROW_PIECE_EDGES``.  Decided once per
+        graph (one read of the largest degree) and cached."""
         holder = self._tables.get("rows")
         if holder is None:
-            rowptr, first, node = self.dst_rowptr, None, None
-            if self.can_split and self.num_edges and int(rowptr.diff().max()) > ROW_SPLIT_EDGES:
-                split = RowSplit(rowptr, ROW_SPLIT_EDGES)
-                first, node = split.first, split.rows
-                piece = torch.arange(split.virtual_rows, device=rowptr.device) - first[node]
-                begin = rowptr[node] + piece * ROW_SPLIT_EDGES
-                rowptr = torch.cat([begin, rowptr[-1:]]).to(torch.int32)
-            holder = self._tables["rows"] = _native.binding().Rows(rowptr, self.num_edges, first, node)
+            rowptr, pieces = self.dst_rowptr, [None] * 4
+            if self.can_split and self.num_edges:
+                degree = rowptr.diff()
+                longest = int(degree.max())
+                if longest > ROW_SPLIT_EDGES or longest > max(ROW_SPLIT_EDGES // 2, 4 * self.num_edges // self.num_nodes):
+                    limit = ROW_SPLIT_EDGES // 2
+                    rowptr, *pieces = _cut_rows(rowptr, degree, limit, ROW_PIECE_EDGES)
+            holder = self._tables["rows"] = _native.binding().Rows(rowptr, self.num_edges, *pieces)
         return holder
 
     def destination_range(self, begin: int, end: int) -> "tuple[LunaTPGraph, int, int]":
@@ -189,6 +195,23 @@ class LunaTPGraph:
         return [self.src, self.dst, self.dst_rowptr, self.src_rowptr, self.edge_ids_by_src,
                 self.source_node_order, self.node_order,
                 seg.nodes, seg.begin, seg.end, seg.rowptr, seg.order, self.node_tiers]
+
+
+def _cut_rows(rowptr: torch.Tensor, degree: torch.Tensor, limit: int, size: int) -> list:
+    """Row pointers with the rows of more than ``limit`` edges cut into pieces of ``size``, and the pieces' tables: the piece of
+    every row (-1: a whole one), and of the pieces their rows, their cut nodes, and where each cut node's begin."""
+    cut = degree > limit
+    count = torch.where(cut, (degree.to(torch.int64) + size - 1) // size, 1)
+    first = torch.cumsum(count, 0) - count
+    node = torch.repeat_interleave(torch.arange(degree.numel(), device=rowptr.device), count)
+    begin = rowptr[node] + (torch.arange(node.numel(), device=rowptr.device) - first[node]) * size
+    is_piece = cut[node]
+    row_of_piece = torch.nonzero(is_piece).squeeze(1)
+    piece_of_row = torch.where(is_piece, torch.cumsum(is_piece, 0) - 1, -1)
+    number = torch.cumsum(cut, 0) - 1  # of a cut node
+    cut_first = torch.cat([count.new_zeros(1), torch.cumsum(count[cut], 0)])
+    return [t.to(torch.int32) for t in (torch.cat([begin, rowptr[-1:]]), piece_of_row, row_of_piece,
+                                        number[node[row_of_piece]], cut_first)]
 
 
 def make_source_segments(src_rowptr: torch.Tensor) -> SourceSegmentTables:

@@ -23,7 +23,7 @@ def _mask(needs) -> int:
 
 
 def _rows(rowptr, edges):
-    return _native.binding().Rows(rowptr, edges, None, None)
+    return _native.binding().Rows(rowptr, edges, None, None, None, None)
 
 
 @torch.library.custom_op("lunaeq::graph_softmax_forward", mutates_args=())

@@ -80,15 +80,40 @@ def test_descriptions_are_checked_at_the_entry_points():
     assert lib.luna_relative_bias_bwd(0, some, some, some, None, 0, 4, 2, 2, None) == _native.LUNA_ERR_SCRATCH
     assert lib.luna_relative_bias_fwd(0, some, some, some, 4, 0, 2, None) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert lib.luna_distance_buckets(2, some, some, 1, some, 1, None) == _native.LUNA_ERR_INVALID_ARGUMENT
-    table = _native.RowTable(2, 4, 2, 16, None, None)
+    table = _native.RowTable(2, 4, 0, 0, 16)
     softmax = lambda t, **k: lib.luna_graph_softmax_fwd(  # noqa: E731
         k.get("dtype", 0), ctypes.byref(t), k.get("logits", some), k.get("table"), None, None, some, k.get("heads", 1), 0, None, 0, None)
     assert softmax(table, heads=0) == softmax(table, dtype=9) == softmax(table, logits=None) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert softmax(table, table=some) == _native.LUNA_ERR_INVALID_ARGUMENT
-    assert softmax(_native.RowTable(2, 4, 2, None, None, None)) == _native.LUNA_ERR_INVALID_ARGUMENT
-    assert softmax(_native.RowTable(2, 1 << 31, 2, 16, None, None)) == _native.LUNA_ERR_OVERFLOW
-    assert softmax(_native.RowTable(2, 4, 2, 16, 16, None)) == _native.LUNA_ERR_INVALID_ARGUMENT
-    assert softmax(_native.RowTable(2, 4, 2, 16, 16, 16)) == _native.LUNA_ERR_SCRATCH
+    assert softmax(_native.RowTable(2, 4, 0, 0, None)) == _native.LUNA_ERR_INVALID_ARGUMENT
+    assert softmax(_native.RowTable(2, 1 << 31, 0, 0, 16)) == _native.LUNA_ERR_OVERFLOW
+    assert softmax(_native.RowTable(2, 4, 2, 1, 16, 16, 16)) == _native.LUNA_ERR_INVALID_ARGUMENT
+    assert softmax(_native.RowTable(2, 4, 3, 1, 16, 16, 16, 16, 16)) == _native.LUNA_ERR_INVALID_ARGUMENT
+    assert softmax(_native.RowTable(2, 4, 2, 1, 16, 16, 16, 16, 16)) == _native.LUNA_ERR_SCRATCH
+
+
+def test_rows_are_cut():
+    """The tables of cut rows, checked against the rows they are made of."""
+    from lunaequivariance_b200.graph import _cut_rows
+
+    for degrees in ([3, 20, 0, 8, 9, 0], [17], [0, 16, 16, 33]):
+        degree = torch.tensor(degrees, dtype=torch.int32)
+        rowptr = torch.cat([torch.zeros(1), degree.cumsum(0)]).to(torch.int32)
+        rows, piece_of_row, row_of_piece, cut_of_piece, cut_first = (t.tolist() for t in _cut_rows(rowptr, degree, 8, 4))
+        row, piece, cut = 0, 0, 0
+        for node, n in enumerate(degrees):
+            count = -(-n // 4) if n > 8 else 1
+            for j in range(count):
+                assert rows[row] == rowptr[node] + 4 * j
+                assert piece_of_row[row] == (piece if n > 8 else -1)
+                if n > 8:
+                    assert (row_of_piece[piece], cut_of_piece[piece]) == (row, cut)
+                    piece += 1
+                row += 1
+            if n > 8:
+                cut += 1
+                assert cut_first[cut] == piece
+        assert rows[row] == sum(degrees) and len(rows) == row + 1 and len(cut_first) == cut + 1 and len(row_of_piece) == piece
 
 
 def test_the_oracle():
