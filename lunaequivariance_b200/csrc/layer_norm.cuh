@@ -90,8 +90,11 @@ struct Place {
   A* exchange;
   unsigned char* shared;
   int turn = 0, stage = 0;
+  const T* coming[IN];                        // chunks: where the next round to be asked for begins, and
+  int64_t rest;                               // the rows from there on
 
-  __device__ __forceinline__ Place(const Block& B_, unsigned char* shared_, A* exchange_) : B(B_), exchange(exchange_), shared(shared_) {
+  __device__ __forceinline__ Place(const Params& P, const Block& B_, const T* const (&arrays)[IN], unsigned char* shared_, A* exchange_)
+      : B(B_), exchange(exchange_), shared(shared_) {
     const int in_cta = threadIdx.x >> 5;
     lane = threadIdx.x & (LANES - 1);
     warps = LANES == 32 ? B.lanes >> 5 : 1;
@@ -100,6 +103,12 @@ struct Place {
     teams = LANES == 32 ? (blockDim.x >> 5) / warps : blockDim.x / LANES;
     begin = warp * kPiece;
     left = B.length - begin - lane * VEC;
+    if (MODE == kChunks) {
+      const int64_t first = static_cast<int64_t>(blockIdx.x - B.first_cta) * teams;
+      rest = P.rows - first;
+#pragma unroll
+      for (int a = 0; a < IN; ++a) coming[a] = arrays[a] ? arrays[a] + first * B.length : nullptr;
+    }
   }
   // Teams before this one whose loop this team shares: those of a warp, or of the CTA where it moves rows together.
   __device__ __forceinline__ int ahead() const { return MODE == kChunks ? team : LANES == 32 ? 0 : (threadIdx.x & 31) / LANES; }
@@ -118,36 +127,42 @@ struct Place {
       for (int c = 0; c < VEC; ++c) to[k][c] = p && in(k) ? rows::widen(p[offset + channel(column(k) + c)]) : otherwise;
   }
 
-  // Starts the copies of a round of rows, of which `row` is this team's, from arrays of P.rows rows.
+  // Starts the copies of a round of rows, of which `row` is this team's, from arrays of P.rows rows.  Rounds are asked for in order.
   __device__ __forceinline__ void request(const Params& P, const T* const (&arrays)[IN], int64_t row) {
     if (MODE == kDirect) return;
+    if (MODE == kPackets) {
 #pragma unroll
-    for (int a = 0; a < IN; ++a) {
-      if (!arrays[a]) continue;
-      if (MODE == kPackets) {
+      for (int a = 0; a < IN; ++a) {
+        if (!arrays[a]) continue;
         const T* from = arrays[a] + row * P.dim + B.offset + column(0);
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (row < P.rows && in(k)) copy_16_async(packet(stage * IN + a, k), from + k * kStep);
-      } else {
-        const int64_t first = row - team, rest = P.rows - first;
-        if (rest <= 0) continue;
-        const int64_t numbers = (rest < teams ? rest : teams) * B.length;
-        const T* from = arrays[a] + first * B.length;
-        const int shift = shift_of(from), pieces = (shift + static_cast<int>(numbers * sizeof(T)) + 15) >> 4;
-        const unsigned char* base = reinterpret_cast<const unsigned char*>(from) - shift;
+      }
+    } else if (rest > 0) {
+      const int bytes = (rest < teams ? static_cast<int>(rest) : teams) * B.length * static_cast<int>(sizeof(T));
+      const bool inner = rest >= 2 * teams;  // another round behind this one: more than 16 bytes
+      const int64_t next = static_cast<int64_t>(B.ctas) * teams;
+#pragma unroll
+      for (int a = 0; a < IN; ++a) {
+        if (!coming[a]) continue;
+        const int shift = shift_of(coming[a]), pieces = (shift + bytes + 15) >> 4;
+        const unsigned char* base = reinterpret_cast<const unsigned char*>(coming[a]) - shift;
         unsigned char* to = chunk(stage * IN + a);
-        for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-          // the first piece may begin before the array, and the last one end after it; another round is more than 16 bytes
-          if ((i > 0 || first > 0 || shift == 0) && (i + 1 < pieces || rest >= 2 * teams)) {
-            copy_16_async(to + i * 16, base + i * 16);
-          } else {
-            for (int j = i * 16; j < i * 16 + 16; j += static_cast<int>(sizeof(T)))
-              if (j >= shift && j < shift + static_cast<int>(numbers * sizeof(T)))
-                *reinterpret_cast<T*>(to + j) = *reinterpret_cast<const T*>(base + j);
+        // the first piece may begin before the array, and the last one end after it: then what is inside of them, at once
+        const int low = shift == 0 || coming[a] != arrays[a] ? 0 : 1, high = inner ? pieces : pieces - 1;
+        for (int i = threadIdx.x; i < high; i += blockDim.x)
+          if (i >= low) copy_16_async(to + i * 16, base + i * 16);
+        if (low > 0 || !inner) {
+          for (int j = threadIdx.x * static_cast<int>(sizeof(T)); j < 32; j += blockDim.x * static_cast<int>(sizeof(T))) {
+            const int at = j < 16 ? j : high * 16 + j - 16;
+            if ((j < 16 ? low > 0 || high == 0 : !inner && high > 0) && at >= shift && at < shift + bytes)
+              *reinterpret_cast<T*>(to + at) = *reinterpret_cast<const T*>(base + at);
           }
         }
+        coming[a] += next * B.length;
       }
+      rest -= next;
     }
     commit_copies();
     stage ^= 1;
@@ -186,19 +201,20 @@ struct Place {
   }
   // All threads have put their numbers of a round of rows: writes a chunk of output `a` to memory.
   __device__ __forceinline__ void send(const Params& P, int a, T* array, int64_t row) const {
-    const int64_t first = row - team, rest = P.rows - first;
+    const int64_t first = row - team, rows_left = P.rows - first;
     T* to = array + first * B.length;
-    const int shift = shift_of(to), end = shift + static_cast<int>((rest < teams ? rest : teams) * B.length * sizeof(T));
+    const int shift = shift_of(to), end = shift + (rows_left < teams ? static_cast<int>(rows_left) : teams) * B.length * static_cast<int>(sizeof(T));
     unsigned char* base = reinterpret_cast<unsigned char*>(to) - shift;
     const unsigned char* from = chunk(kStages * IN + a);
-    for (int i = threadIdx.x * 16; i < end; i += blockDim.x * 16) {
-      if (i >= shift && i + 16 <= end) {
-        *reinterpret_cast<uint4*>(base + i) = *reinterpret_cast<const uint4*>(from + i);
-      } else {
-        for (int j = i; j < i + 16; j += static_cast<int>(sizeof(T)))
-          if (j >= shift && j < end) *reinterpret_cast<T*>(base + j) = *reinterpret_cast<const T*>(from + j);
+    const int low = shift == 0 ? 0 : 16, high = end & ~15;  // whole pieces; the others number by number
+    for (int i = threadIdx.x * 16; i < high; i += blockDim.x * 16)
+      if (i >= low) *reinterpret_cast<uint4*>(base + i) = *reinterpret_cast<const uint4*>(from + i);
+    if (low > 0 || high < end)
+      for (int j = threadIdx.x * static_cast<int>(sizeof(T)); j < 32; j += blockDim.x * static_cast<int>(sizeof(T))) {
+        const int at = j < 16 ? j : high + j - 16;
+        if ((j < 16 ? low > 0 || high == 0 : high > 0) && at >= shift && at < end)
+          *reinterpret_cast<T*>(base + at) = *reinterpret_cast<const T*>(from + at);
       }
-    }
   }
 
   // Sums over the threads of a row.
@@ -285,9 +301,9 @@ struct Operands {
 template <typename T, int VEC, int K, int LANES, int MODE>
 __device__ __forceinline__ void forward(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
   using A = Acc<T>;
-  Place<T, VEC, K, LANES, MODE, 1, 1> place(B, raw, exchange);
-  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   const T* const arrays[1] = {o.x};
+  Place<T, VEC, K, LANES, MODE, 1, 1> place(P, B, arrays, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   auto request = [&](int64_t row) { place.request(P, arrays, row); };
   int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
   for (int j = 0; j < kStages; ++j) request(row + j * step);
@@ -338,9 +354,9 @@ __device__ __forceinline__ void forward(const Params& P, const Block& B, int ind
 template <typename T, int VEC, int K, int LANES, int MODE>
 __device__ __forceinline__ void backward(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
   using A = Acc<T>;
-  Place<T, VEC, K, LANES, MODE, 2, 1> place(B, raw, exchange);
-  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   const T* const arrays[2] = {o.x, o.g};
+  Place<T, VEC, K, LANES, MODE, 2, 1> place(P, B, arrays, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   auto request = [&](int64_t row) { place.request(P, arrays, row); };
   auto moments = [&](int64_t row) { return row < P.rows ? o.stats_in[index * P.rows + row] : Moments<A>{A(0), A(0)}; };
   int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
@@ -400,9 +416,9 @@ __device__ __forceinline__ void backward(const Params& P, const Block& B, int in
 template <typename T, int VEC, int K, int LANES, int MODE>
 __device__ __forceinline__ void second(const Params& P, const Block& B, int index, const Operands<T>& o, unsigned char* raw, Acc<T>* exchange) {
   using A = Acc<T>;
-  Place<T, VEC, K, LANES, MODE, 3, 2> place(B, raw, exchange);
-  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   const T* const arrays[3] = {o.x, o.g, o.rx};
+  Place<T, VEC, K, LANES, MODE, 3, 2> place(P, B, arrays, raw, exchange);
+  const int64_t step = static_cast<int64_t>(B.ctas) * place.teams;
   auto request = [&](int64_t row) { place.request(P, arrays, row); };
   auto moments = [&](int64_t row) { return row < P.rows ? o.stats_in[index * P.rows + row] : Moments<A>{A(0), A(0)}; };
   int64_t row = static_cast<int64_t>(blockIdx.x - B.first_cta) * place.teams + place.team;
@@ -594,11 +610,9 @@ int launch(Params P, const Call& c, cudaStream_t stream) {
   const size_t sums_bytes = sums ? static_cast<size_t>(THREADS) * K * VEC * sizeof(A) : 0;
   const size_t shared = rows_bytes > sums_bytes ? rows_bytes : sums_bytes;
   const auto kernel = norm_kernel<T, VEC, K, THREADS, MODE, ORDER>;
-  if (shared > 40 * 1024) LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
-  int resident = 0;
-  LUNA_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, THREADS, shared));
-  resident *= rows::processors();
-  if (resident < 1) return fail(LUNA_ERR_CUDA, "layer norm does not fit the current device");
+  static rows::Kernel known;
+  const int resident = known.resident(kernel, THREADS, shared);
+  if (resident < 1) return resident;
   const int ctas = assign(P, THREADS, resident);
   const Operands<T> o{in(c.x), in(c.weight), in(c.bias), in(c.g), in(c.rx), in(c.rw), in(c.rb), static_cast<const Moments<A>*>(c.stats_in),
                       out(c.y), out(c.gx), out(c.hx), out(c.hg), static_cast<Moments<A>*>(c.stats_out),

@@ -238,7 +238,8 @@ int table_gradient(const T* g, const int32_t* buckets, T* gtable, void* scratch,
   // more edges under way where a multiprocessor has few threads
   constexpr int kMany = VEC * sizeof(A) > 16 ? 8 : 16;  // packets of eight: the registers of eight edges are all
   const auto kernel = cut.threads > 128 ? table_kernel<T, VEC, 8> : table_kernel<T, VEC, kMany>;
-  if (cut.shared > 40 * 1024) LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cut.shared)));
+  static rows::Kernel known[2];
+  if (const int status = known[cut.threads > 128].allow(kernel, static_cast<size_t>(cut.shared))) return status;
   kernel<<<dim3(cut.parts_of_edges, cut.parts_of_heads, cut.parts_of_buckets), cut.threads, cut.shared, stream>>>(
       g, buckets, partial, edges, static_cast<int>(num_buckets), static_cast<int>(heads), cut, aligned_to(buckets, 16));
   LUNA_LAUNCH_CHECK("gradient of the bias table");

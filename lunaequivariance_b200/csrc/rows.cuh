@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.h"
 
 namespace luna {
@@ -73,13 +75,57 @@ inline int next_power_of_two(int64_t v) {
   return p;
 }
 
+constexpr int kMostDevices = 64;
+// The current device; -1 if it cannot be asked, or is beyond those that things are remembered for.
+inline int current_device() {
+  int device = -1;
+  return cudaGetDevice(&device) == cudaSuccess && device < kMostDevices ? device : -1;
+}
 // Multiprocessors of the current device; 0 if it cannot be asked.
 inline int processors() {
-  int device = 0, count = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return 0;
+  static std::atomic<int> known[kMostDevices];
+  const int device = current_device();
+  if (device < 0) return 0;
+  int count = known[device].load(std::memory_order_relaxed);
+  if (count) return count;
   if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  known[device].store(count, std::memory_order_relaxed);
   return count;
 }
+
+// What is known of a kernel, so that a launch does not ask the runtime again: on which devices it may use as much shared memory
+// as there is (always all of it, so that calls of other shapes on other threads change nothing), and how many CTAs are resident
+// with the shared memory of the last call.
+struct Kernel {
+  std::atomic<uint64_t> allowed{0}, last{0};
+
+  template <typename... P>
+  int allow(void (*kernel)(P...), size_t shared) {
+    const int device = current_device();
+    if (device < 0) return fail(LUNA_ERR_CUDA, "the current device is unknown");
+    if (shared > kMostShared) return fail(LUNA_ERR_UNSUPPORTED, "%zu bytes of shared memory", shared);
+    if (!(allowed.load(std::memory_order_acquire) >> device & 1)) {
+      LUNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)));
+      allowed.fetch_or(1ull << device, std::memory_order_release);
+    }
+    return LUNA_OK;
+  }
+  // CTAs on the whole device, or less than one (a status).
+  template <typename... P>
+  int resident(void (*kernel)(P...), int threads, size_t shared) {
+    if (const int status = allow(kernel, shared)) return status;
+    const uint64_t key = (static_cast<uint64_t>(shared) << 6 | current_device()) << 16;
+    const uint64_t known = last.load(std::memory_order_relaxed);
+    if (known && (known >> 16 << 16) == key) return static_cast<int>(known & 0xffff);
+    int count = 0;
+    LUNA_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&count, kernel, threads, shared));
+    count *= processors();
+    if (count < 1 || count > 0xffff) return fail(LUNA_ERR_CUDA, "a kernel does not fit the current device");
+    last.store(key | static_cast<uint64_t>(count), std::memory_order_relaxed);
+    return count;
+  }
+  static constexpr size_t kMostShared = 216 * 1024;  // beside what the kernels have at compile time
+};
 
 }  // namespace rows
 }  // namespace luna
