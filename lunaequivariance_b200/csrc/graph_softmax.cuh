@@ -257,14 +257,24 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
   const int batch = K * slots;
   const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
   const int64_t count = PHASE == kApply ? R.pieces : R.count;
-  for (int64_t number = static_cast<int64_t>(blockIdx.x) * teams + team; number - ahead < count; number += step) {
-    int first = 0, length = 0, piece = -1;
+  // Where a row is, one row ahead of its use: of three trips to memory that follow one another the first
+  int next_first = 0, next_length = 0, next_piece = -1;
+  auto find = [&](int64_t number) {
+    next_first = next_length = 0;
+    next_piece = -1;
     if (number < count && here) {
       const int64_t row = PHASE == kApply ? R.row_of_piece[number] : number;
-      if constexpr (PHASE == kMixed) piece = R.piece_of_row[row];
-      first = R.rowptr[row];
-      length = R.rowptr[row + 1] - first;
+      if constexpr (PHASE == kMixed) next_piece = R.piece_of_row[row];
+      next_first = R.rowptr[row];
+      next_length = R.rowptr[row + 1];
     }
+  };
+  int64_t number = static_cast<int64_t>(blockIdx.x) * teams + team;
+  find(number);
+  for (; number - ahead < count; number += step) {
+    int first = next_first;
+    const int length = next_length - next_first, piece = next_piece;
+    find(number + step);
     first += slot;
     const int left = length - slot;
     const int behind = length > 0 ? (length - 1) / batch * batch : 0;  // where the last batch begins
@@ -386,16 +396,24 @@ join_kernel(const Rows R, int heads, int across, Pair<A>* __restrict__ stats) {
 
 template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES = 0>
 int start(const Rows& R, const Shape& S, const Operands<T>& o, Pair<Acc<T>>* stats, cudaStream_t stream) {
-  const int64_t ctas = ceil_div(PHASE == kApply ? R.pieces : R.count, kThreads / S.lanes), most = static_cast<int64_t>(rows::processors()) * 256;
-  const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most), static_cast<unsigned>(ceil_div(S.heads, S.across * VEC)));
-  rows_kernel<T, VEC, K, ORDER, PHASE, LANES><<<grid, kThreads, 0, stream>>>(R, S, o, stats);
+  // As many CTAs as are resident, which go from row to row: 2.6 M edges with 8 heads, forward 59 -> 46 us.  Rows of very different
+  // length are handed out by the hardware instead: 1.0 M edges of hubs with 3 heads, FP64, 33 us, and 43 from row to row.
+  const auto kernel = rows_kernel<T, VEC, K, ORDER, PHASE, LANES>;
+  static rows::Kernel known;
+  const int resident = known.resident(kernel, kThreads, 0);
+  if (resident < 1) return resident;
+  const int64_t parts = ceil_div(S.heads, S.across * VEC);
+  const int64_t ctas = ceil_div(PHASE == kApply ? R.pieces : R.count, kThreads / S.lanes), most = PHASE == kMixed ? ctas : resident > parts ? resident / parts : 1;
+  kernel<<<dim3(static_cast<unsigned>(ctas < most ? ctas : most), static_cast<unsigned>(parts)), kThreads, 0, stream>>>(R, S, o, stats);
   LUNA_LAUNCH_CHECK("softmax over in-edges");
   return LUNA_OK;
 }
 
 template <typename T, int VEC, int ORDER>
 int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch, cudaStream_t stream) {
-  constexpr int K = VEC * sizeof(Acc<T>) >= 32 ? 2 : VEC * sizeof(Acc<T>) >= 16 ? 4 : 8;
+  // Sixteen numbers of a thread in registers; single ones, with their exponentials and addresses, spill (forward, 2.6 M edges
+  // with one head: 23 us, with eight 14; the backward has room: 8.3 and 9.8).
+  constexpr int K = sizeof(T) > 4 ? 8 / VEC : VEC == 1 && ORDER != kBackward ? 8 : 16 / VEC;
   Shape S{};
   S.heads = static_cast<int>(heads);
   S.num_buckets = static_cast<int>(num_buckets);
@@ -409,6 +427,7 @@ int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, con
   if (!R.pieces) {
     if (S.across * VEC == S.heads && S.lanes == 32) return start<T, VEC, K, ORDER, kWhole, 32>(R, S, o, stats, stream);
     if (S.across * VEC == S.heads && S.lanes == 16) return start<T, VEC, K, ORDER, kWhole, 16>(R, S, o, stats, stream);
+    if (S.across * VEC == S.heads && S.lanes == 8) return start<T, VEC, K, ORDER, kWhole, 8>(R, S, o, stats, stream);
     return start<T, VEC, K, ORDER, kWhole>(R, S, o, stats, stream);
   }
   if (const int status = start<T, VEC, K, ORDER, kMixed>(R, S, o, stats, stream)) return status;

@@ -101,6 +101,7 @@ struct Kernel {
 
   template <typename... P>
   int allow(void (*kernel)(P...), size_t shared) {
+    if (shared <= 32 * 1024) return LUNA_OK;  // with what it has at compile time within the 48 KB that every kernel may use
     const int device = current_device();
     if (device < 0) return fail(LUNA_ERR_CUDA, "the current device is unknown");
     if (shared > kMostShared) return fail(LUNA_ERR_UNSUPPORTED, "%zu bytes of shared memory", shared);
