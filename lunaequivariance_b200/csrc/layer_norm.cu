@@ -48,6 +48,11 @@ int checked(const luna_norm_desc* desc, const void* p, const char* name, bool re
   return aligned_to(p, rows::size_of(desc->dtype)) ? LUNA_OK : fail(LUNA_ERR_MISALIGNED, "%s is not aligned to its element size", name);
 }
 
+int checked_stats(const luna_norm_desc* desc, const void* stats, bool required) {
+  if (!stats) return required ? fail(LUNA_ERR_INVALID_ARGUMENT, "stats is null") : LUNA_OK;
+  return aligned_to(stats, 2 * rows::acc_size_of(desc->dtype)) ? LUNA_OK : fail(LUNA_ERR_MISALIGNED, "stats is not aligned to a pair");
+}
+
 int dispatch(Order order, const luna_norm_desc* desc, const Params& P, const Call& o, void* stream) {
   int status = LUNA_OK;
   rows::with_type(desc->dtype, [&](auto zero) { status = run<decltype(zero)>(order, P, o, static_cast<cudaStream_t>(stream)); });
@@ -90,6 +95,7 @@ extern "C" int luna_layer_norm_fwd(const luna_norm_desc* desc, const void* x, co
   LUNA_TRY(checked(desc, y, "y", rows > 0));
   LUNA_TRY(checked(desc, weight, "weight", false));
   LUNA_TRY(checked(desc, bias, "bias", false));
+  LUNA_TRY(checked_stats(desc, stats, false));
   if (rows == 0) return LUNA_OK;
   Call o{};
   o.x = x, o.weight = weight, o.bias = bias, o.y = y, o.stats_out = stats;
@@ -108,7 +114,7 @@ extern "C" int luna_layer_norm_bwd(const luna_norm_desc* desc, const void* x, co
   LUNA_TRY(checked(desc, gx, "gx", false));
   LUNA_TRY(checked(desc, gw, "gw", false));
   LUNA_TRY(checked(desc, gb, "gb", false));
-  if (rows > 0 && !stats) return luna::fail(LUNA_ERR_INVALID_ARGUMENT, "stats is null");
+  LUNA_TRY(checked_stats(desc, stats, rows > 0));
   if (!gw && !gb && (!gx || rows == 0)) return LUNA_OK;
   Call o{};
   o.x = x, o.weight = weight, o.stats_in = stats, o.g = g, o.gx = gx, o.gw = gw, o.gb = gb, o.scratch = scratch,
@@ -133,7 +139,7 @@ extern "C" int luna_layer_norm_dbl_bwd(const luna_norm_desc* desc, const void* x
   LUNA_TRY(checked(desc, hx, "hx", false));
   LUNA_TRY(checked(desc, hw, "hw", false));
   LUNA_TRY(checked(desc, hg, "hg", false));
-  if (rows > 0 && !stats) return luna::fail(LUNA_ERR_INVALID_ARGUMENT, "stats is null");
+  LUNA_TRY(checked_stats(desc, stats, rows > 0));
   if (!hw && ((!hx && !hg) || rows == 0)) return LUNA_OK;
   Call o{};
   o.x = x, o.weight = weight, o.stats_in = stats, o.g = g, o.rx = rx, o.rw = rw, o.rb = rb, o.hx = hx, o.gw = hw, o.hg = hg,

@@ -15,12 +15,13 @@
 // launch, in an order that only the sizes decide: no atomics, the same bits every time.
 //
 // Rows arrive in shared memory by asynchronous copies, one round ahead of their use, so that the memory is busy while sums
-// are made.  Where rows are aligned, each thread copies what it will read itself and waits for nobody.  Rows that begin
-// anywhere in 16 bytes are moved a CTA's round of rows at a time, one contiguous chunk in aligned pieces, and read and written
-// number by number in shared memory (600,000 rows of 50 floats, forward: 77 us when global memory was read so).
-// Rows wider than a CTA of 256 holds, and unaligned blocks between others, are read when they are wanted.
+// are made.  Each thread copies what it will read itself, in the widest packets that the rows allow, and waits for nobody.  16-bit
+// rows of an odd length, which no asynchronous copy can begin at, are moved a CTA's round of rows at a time, one contiguous chunk
+// in aligned pieces, and read and written number by number in shared memory (20,011 rows of 1001 BF16: forward 77 -> 50 us, backward 75
+// -> 59).  Rows wider than a CTA of 256 holds, and such rows of several blocks, are read when they are wanted.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -63,8 +64,13 @@ struct Moments {
   A mean, scale;
 };
 
-__device__ __forceinline__ void copy_16_async(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const unsigned address = static_cast<unsigned>(__cvta_generic_to_shared(to));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(address), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(address), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -82,6 +88,7 @@ constexpr int kStages = 2;  // rounds of rows on their way
 template <typename T, int VEC, int K, int LANES, int MODE, int IN, int OUT>
 struct Place {
   using A = Acc<T>;
+  static constexpr int kBytes = MODE == kPackets ? VEC * static_cast<int>(sizeof(T)) : 16;  // of a copy: 4, 8 or 16
   static constexpr int kStep = LANES * VEC;   // from one of a thread's packets to the next
   static constexpr int kPiece = kStep * K;    // columns of a warp
   const Block& B;
@@ -116,7 +123,7 @@ struct Place {
   __device__ __forceinline__ int column(int k) const { return begin + lane * VEC + k * kStep; }
   __device__ __forceinline__ int channel(int i) const { return B.components == 1 ? i : static_cast<int>(__umulhi(i, B.inverse)); }
   // Packets: a thread's own, those of a warp's threads side by side.  Chunks: one array's after the other's.
-  __device__ __forceinline__ unsigned char* packet(int array, int k) const { return shared + ((array * K + k) * blockDim.x + threadIdx.x) * 16; }
+  __device__ __forceinline__ unsigned char* packet(int array, int k) const { return shared + ((array * K + k) * blockDim.x + threadIdx.x) * kBytes; }
   __device__ __forceinline__ unsigned char* chunk(int array) const { return shared + array * B.chunk; }
   static __device__ __forceinline__ int shift_of(const T* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15); }
 
@@ -137,7 +144,7 @@ struct Place {
         const T* from = arrays[a] + row * P.dim + B.offset + column(0);
 #pragma unroll
         for (int k = 0; k < K; ++k)
-          if (row < P.rows && in(k)) copy_16_async(packet(stage * IN + a, k), from + k * kStep);
+          if (row < P.rows && in(k)) copy_async<kBytes>(packet(stage * IN + a, k), from + k * kStep);
       }
     } else if (rest > 0) {
       const int bytes = (rest < teams ? static_cast<int>(rest) : teams) * B.length * static_cast<int>(sizeof(T));
@@ -152,7 +159,7 @@ struct Place {
         // the first piece may begin before the array, and the last one end after it: then what is inside of them, at once
         const int low = shift == 0 || coming[a] != arrays[a] ? 0 : 1, high = inner ? pieces : pieces - 1;
         for (int i = threadIdx.x; i < high; i += blockDim.x)
-          if (i >= low) copy_16_async(to + i * 16, base + i * 16);
+          if (i >= low) copy_async<16>(to + i * 16, base + i * 16);
         if (low > 0 || !inner) {
           for (int j = threadIdx.x * static_cast<int>(sizeof(T)); j < 32; j += blockDim.x * static_cast<int>(sizeof(T))) {
             const int at = j < 16 ? j : high * 16 + j - 16;
@@ -606,9 +613,9 @@ int launch(Params P, const Call& c, cudaStream_t stream) {
   // Room for the rows on their way and on their way out, and later for the sums of the CTA's threads
   constexpr int in_arrays = ORDER == kForward ? 1 : ORDER == kBackward ? 2 : 3, out_arrays = ORDER == kSecond ? 2 : 1;
   const size_t chunk = lay_out<T>(P, VEC, K, THREADS);
-  const size_t rows_bytes = MODE == kDirect ? 0 : MODE == kPackets ? kStages * in_arrays * K * THREADS * 16 : (kStages * in_arrays + out_arrays) * chunk;
+  const size_t rows_bytes = MODE == kDirect ? 0 : MODE == kPackets ? kStages * in_arrays * K * VEC * sizeof(T) * THREADS : (kStages * in_arrays + out_arrays) * chunk;
   const size_t sums_bytes = sums ? static_cast<size_t>(THREADS) * K * VEC * sizeof(A) : 0;
-  const size_t shared = rows_bytes > sums_bytes ? rows_bytes : sums_bytes;
+  const size_t shared = std::max(rows_bytes, sums_bytes);
   const auto kernel = norm_kernel<T, VEC, K, THREADS, MODE, ORDER>;
   static rows::Kernel known;
   const int resident = known.resident(kernel, THREADS, shared);
@@ -630,39 +637,60 @@ int launch(Params P, const Call& c, cudaStream_t stream) {
   return LUNA_OK;
 }
 
+// Packets narrower than sixteen bytes.  Numbers of a thread, measured, forward / backward in us for four, eight or sixteen: 600,000 rows
+// of 50x0e, FP32 (packets of two) 55 / 78, 43 / 72, 46 / 76, BF16 56 / 80, 41 / 67, 37 / 59; 20,000 of 1001x0e, FP32 (single numbers)
+// 55 / 64, 39 / 67, 44 / 72; 300,000 of 51x0e, FP64, four or eight 44 / 69 / 110 (second order) and 48 / 75 / 159.
+template <typename T, int VEC, int ORDER>
+int with_packets(const Params& P, int64_t longest, bool few, const Call& c, cudaStream_t stream) {
+  constexpr int kFew = VEC < 4 ? 4 / VEC : 1, kMany = (sizeof(T) == 2 && ORDER != kSecond ? 16 : 8) / VEC;
+  const int64_t n = longest / VEC;
+  if ((few || sizeof(T) > 4 || longest <= 16) && n <= kThreads * kFew) return launch<T, VEC, kFew, kThreads, kPackets, ORDER>(P, c, stream);
+  if (n <= kThreads * kMany) return launch<T, VEC, kMany, kThreads, kPackets, ORDER>(P, c, stream);
+  return launch<T, VEC, 16 / VEC, kWideThreads, kDirect, ORDER>(P, c, stream);
+}
+
 template <typename T, int ORDER>
 int choose(const Params& P, const Call& c, cudaStream_t stream) {
-  constexpr int kPacket = 16 / static_cast<int>(sizeof(T));
-  bool packets = P.dim % kPacket == 0;
+  constexpr int kWidest = 16 / static_cast<int>(sizeof(T));
   int64_t longest = 0;
+  int vec = kWidest;  // numbers of a packet: at most 16 bytes, at least the four of an asynchronous copy
   for (int i = 0; i < P.blocks; ++i) {
-    packets = packets && P.block[i].offset % kPacket == 0 && P.block[i].length % kPacket == 0;
+    while (vec > 1 && (P.dim % vec || P.block[i].offset % vec || P.block[i].length % vec)) vec >>= 1;
     longest = P.block[i].length > longest ? P.block[i].length : longest;
   }
   for (const void* p : {c.x, c.g, c.rx, static_cast<const void*>(c.y), static_cast<const void*>(c.gx), static_cast<const void*>(c.hx),
                         static_cast<const void*>(c.hg)})
-    packets = packets && aligned_to(p, 16);
+    while (vec > 1 && !aligned_to(p, vec * sizeof(T))) vec >>= 1;
   // Packets of a thread.  More of them mean fewer threads per row, so fewer steps for its sums and no barrier, as long as the
   // registers allow it.  Measured, forward / backward / second order in us: 50,000 rows of 128x0e+128x1o+128x2e, FP32, one, two
   // or four packets 139 / 199, 87 / 168, 84 / 123; 100,000 of 64x0e+64x1o+64x2e 139 / 180 / 336, 86 / 163 / 235, 82 / 123 / 287;
   // 86,000 of 64x0e 10.9 / 13.0, 8.9 / 14.9, 9.7 / 15.4; 40,000 of 1024x0e, BF16, 58 / 76, 55 / 63, 54 / 79.  Where there are not
   // enough rows to fill the GPU, the threads are: 24 rows 2.6, 2.8 and 3.6 us, 500 rows of 64x0e 2.6 / 3.1, 3.1 / 4.2, 4.0 / 5.7.
-  const bool few = P.rows * P.dim <= static_cast<int64_t>(rows::processors()) * 1024 * (packets ? kPacket : 1);
-  if (packets) {
-    const int64_t n = longest / kPacket;
+  const bool few = P.rows * P.dim <= static_cast<int64_t>(rows::processors()) * 1024 * (vec == kWidest ? kWidest : 1);
+  if (vec == kWidest) {
+    const int64_t n = longest / kWidest;
     const int64_t most_of_two = ORDER == kSecond || sizeof(T) == 2 ? kThreads * 2 : 64;
-    if (few && n <= kThreads) return launch<T, kPacket, 1, kThreads, kPackets, ORDER>(P, c, stream);
-    if (n <= most_of_two) return launch<T, kPacket, 2, kThreads, kPackets, ORDER>(P, c, stream);
-    if (n <= kThreads * 4) return launch<T, kPacket, 4, kThreads, kPackets, ORDER>(P, c, stream);
-    if (n <= kWideThreads * 4) return launch<T, kPacket, 4, kWideThreads, kDirect, ORDER>(P, c, stream);
+    if (few && n <= kThreads) return launch<T, kWidest, 1, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= most_of_two) return launch<T, kWidest, 2, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= kThreads * 4) return launch<T, kWidest, 4, kThreads, kPackets, ORDER>(P, c, stream);
+    if (n <= kWideThreads * 4) return launch<T, kWidest, 4, kWideThreads, kDirect, ORDER>(P, c, stream);
+    return launch<T, 1, 16, kWideThreads, kDirect, ORDER>(P, c, stream);
   }
-  constexpr int kMost = sizeof(T) > 4 ? 8 : 16;  // numbers of a thread
-  if (longest <= kThreads * kMost) {
-    if (P.blocks > 1) return launch<T, 1, kMost, kThreads, kDirect, ORDER>(P, c, stream);
-    if (few && longest <= kThreads * 4) return launch<T, 1, 4, kThreads, kChunks, ORDER>(P, c, stream);
-    return launch<T, 1, kMost, kThreads, kChunks, ORDER>(P, c, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 4) return with_packets<T, 4, ORDER>(P, longest, few, c, stream);
+    if (vec == 2) return with_packets<T, 2, ORDER>(P, longest, few, c, stream);
+    if (longest <= kThreads * 16) {
+      if (P.blocks > 1) return launch<T, 1, 16, kThreads, kDirect, ORDER>(P, c, stream);
+      if (few && longest <= kThreads * 4) return launch<T, 1, 4, kThreads, kChunks, ORDER>(P, c, stream);
+      return launch<T, 1, 16, kThreads, kChunks, ORDER>(P, c, stream);
+    }
+    return launch<T, 1, 16, kWideThreads, kDirect, ORDER>(P, c, stream);
+  } else {
+    if constexpr (sizeof(T) == 4) {
+      if (vec == 2) return with_packets<T, 2, ORDER>(P, longest, few, c, stream);
+    }
+    return with_packets<T, 1, ORDER>(P, longest, few, c, stream);
   }
-  return launch<T, 1, 16, kWideThreads, kDirect, ORDER>(P, c, stream);
 }
 
 template <typename T>

@@ -1237,25 +1237,25 @@ PYBIND11_MODULE(luna_torch, m) {
   m.def("distance_buckets", torch::wrap_pybind_function(distance_buckets));
   m.def("relative_bias", torch::wrap_pybind_function(relative_bias));
   m.def("graph_softmax", torch::wrap_pybind_function(graph_softmax));
-  m.def("layer_norm_forward", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Maybe& bias) {
+  m.def("layer_norm_forward", torch::wrap_pybind_function([](const NormPtr& n, const Tensor& x, const Maybe& weight, const Maybe& bias) {
     return listed(norm_forward(*n, x, of(weight), of(bias), true));
-  });
-  m.def("layer_norm_backward", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g, int mask) {
+  }));
+  m.def("layer_norm_backward", torch::wrap_pybind_function([](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g, int mask) {
     return listed(norm_backward(*n, x, of(weight), stats, g, mask));
-  });
-  m.def("layer_norm_double", [](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g,
+  }));
+  m.def("layer_norm_double", torch::wrap_pybind_function([](const NormPtr& n, const Tensor& x, const Maybe& weight, const Tensor& stats, const Tensor& g,
                                 const Maybe& rx, const Maybe& rw, const Maybe& rb, int mask) {
     return listed(norm_double(*n, x, of(weight), stats, g, of(rx), of(rw), of(rb), mask));
-  });
+  }));
   m.def("relative_bias_forward", torch::wrap_pybind_function(bias_forward));
   m.def("relative_bias_backward", torch::wrap_pybind_function(bias_backward));
-  m.def("graph_softmax_forward", [](const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
+  m.def("graph_softmax_forward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
     return softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
-  });
-  m.def("graph_softmax_backward", [](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
-                                     int mask) { return listed(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, mask)); });
-  m.def("graph_softmax_double", [](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
+  }));
+  m.def("graph_softmax_backward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
+                                     int mask) { return listed(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, mask)); }));
+  m.def("graph_softmax_double", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
                                    const Maybe& rtable, int mask) {
     return listed(softmax_double(*rows, alpha, g, of(buckets), of(r), of(rtable), mask));
-  });
+  }));
 }

@@ -104,7 +104,9 @@ def graph_softmax(logits, graph, *, mask=None, table=None, buckets=None):
     ``table[buckets, heads]`` (of the type of the logits) and ``buckets[edges]`` (int32, as from ``distance_buckets``)
     add a learned bias to the logits; a bucket that is no row of the table adds nothing.  ``mask[edges]`` (bool) keeps the
     edges that are ``True``; what stands in the others' logits does not matter, and their result is zero.  A node whose
-    edges are all masked, or have logits of minus infinity only, gets zeros.
+    edges are all masked, or have logits of minus infinity only, gets zeros.  Where the result is zero nothing flows back.
+
+    The first call with a graph reads its largest degree; make it before a CUDA graph is captured.
     """
     if not isinstance(graph, LunaTPGraph):
         raise TypeError("graph must come from make_graph")

@@ -180,6 +180,50 @@ def test_infinities_that_are_not_masked():
     assert luna.graph_softmax(nan_only, graph).isnan().all()
 
 
+def test_values_beyond_32_bits():
+    """More than 2^31 logits: the last rows are what they are in a small graph."""
+    nodes, degree, heads = 34_000, 1000, 64
+
+    def run(nodes, logits, g):
+        dst = torch.arange(nodes, device=DEVICE).repeat_interleave(degree)
+        graph = luna.make_graph(torch.zeros_like(dst), dst, nodes)
+        z = logits.requires_grad_(True)
+        alpha = luna.graph_softmax(z, graph)
+        return alpha.detach()[-2 * degree:], torch.autograd.grad(alpha, z, g)[0][-2 * degree:]
+
+    generator = torch.Generator(device=DEVICE).manual_seed(0)
+    tail, gtail = (torch.randn(5 * degree, heads, generator=generator, device=DEVICE).to(BF16) for _ in range(2))
+    logits = torch.zeros(nodes * degree, heads, device=DEVICE, dtype=BF16)
+    assert logits.numel() > 1 << 31
+    g = torch.zeros_like(logits)
+    logits[-5 * degree:], g[-5 * degree:] = tail, gtail
+    for a, b in zip(run(nodes, logits, g), run(5, tail.clone(), gtail)):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap share nothing."""
+    graph, _, _, p = problem("even", 8, 16, 0.1, F32)
+    long, _, _, q = problem("long", 8, 16, 0.1, F32)
+    problems = [(graph, {k: None if v is None else v.to(DEVICE) for k, v in p.items()}),
+                (long, {k: None if v is None else v.to(DEVICE) for k, v in q.items()})]
+
+    def step(graph, p):
+        return derivatives(lambda z, t: luna.graph_softmax(z, graph, mask=p["mask"], table=t, buckets=p["buckets"]), p)
+
+    want = [step(*x) for x in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    found = []
+    for _ in range(10):
+        for stream, x in zip(streams, problems):
+            with torch.cuda.stream(stream):
+                found.append(step(*x))
+    torch.cuda.synchronize()
+    for i, f in enumerate(found):
+        assert all(torch.equal(f[k], want[i % 2][k]) for k in f)
+
+
 def test_memory_orders():
     generator = torch.Generator(device=DEVICE).manual_seed(0)
     graph, dst = graph_of([40] * 30, torch.Generator().manual_seed(0))

@@ -159,6 +159,27 @@ def test_without_parameters(parts):
         close(a, c, F32, 10 * c.abs().max(), k)
 
 
+@pytest.mark.parametrize("slot", [0, 1, 2])
+@pytest.mark.parametrize("irreps,dtype", [("64x0e+16x1o", F64), ("51x0e", F64), ("33x0e", BF16)])
+def test_second_order_of_one_gradient(irreps, dtype, slot):
+    """The cotangent of gx, of gw or of gb alone."""
+    config, p = problem(irreps, 70, dtype)
+
+    def run(norm, p):
+        x, w, b, g = (p[k].clone().requires_grad_(True) for k in ("x", "weight", "bias", "g"))
+        first = torch.autograd.grad(norm(x, w, b), (x, w, b), g, create_graph=True)[slot]
+        return [t for t in torch.autograd.grad(first, (x, w, g), p[("rx", "rw", "rb")[slot]], allow_unused=True)]
+
+    want = run(lambda x, w, b: oracle.layer_norm(x, irreps, w, b), {k: v.double() for k, v in p.items()})
+    got = run(lambda x, w, b: luna.layer_norm(x, irreps, w, b), {k: v.to(DEVICE) for k, v in p.items()})
+    bounds = sizes(config, p)
+    for k, a, b in zip(("hx", "hw", "hg"), got, want):
+        if b is None:  # the definition has no path there: a derivative of zero
+            assert a is None or not a.any(), k
+        else:
+            close(a, b, dtype, bounds[k], k)
+
+
 def test_gradient_against_differences():
     irreps = "6x0e+3x1o+2x2e"
     config, p = problem(irreps, 4, F64)

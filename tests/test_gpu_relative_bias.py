@@ -152,6 +152,7 @@ def test_module_compile_and_capture():
         # no graph is left behind: the autograd engine cannot capture a backward pass while an eager graph of the leaf lives
         return bias.detach(), torch.autograd.grad((bias ** 2).sum(), table)[0]
 
+    assert torch.equal(torch.compile(module, fullgraph=True)(vec.double()), module(vec.double()))
     traced = torch.compile(lambda t, v: luna.relative_bias(t, luna.distance_buckets(v, borders)), fullgraph=True)
     eager = gradient(table, vec)
     assert torch.equal(traced(table, vec), eager[0])
