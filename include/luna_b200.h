@@ -301,7 +301,10 @@ LUNA_API int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* buc
  * row's piece, or -1; row_of_piece and cut_of_piece lead back.  Without cut nodes the four tables are null.
  *
  * forward:  alpha = softmax(logits + table[buckets]) over the unmasked edges of each node (mask[e] = 0: left out, alpha 0);
- *           a node without any, or with logits of -inf only, gets zeros.  table, buckets, mask may be null.
+ *           a node without any, or with logits of -inf only, gets zeros.  table, buckets, mask may be null.  For the 16-bit
+ *           types `wide`, if not null, gets alpha in float as well; the other types ignore it.
+ * alpha, as the other two take it, is in float for the 16-bit types (what `wide` got) and in the type itself for the others:
+ * gradients by bucket are sums of differences, in which the rounding of alpha would count many times.
  * backward: glogits = alpha (g - sum alpha g), and gtable its sums by bucket (null: not wanted).  Where alpha is zero the
  *           gradient is zero, whatever stands in g there.
  * second:   with r, rtable the cotangents of glogits, gtable (null: zero), the derivatives with respect to alpha and g;
@@ -317,7 +320,7 @@ typedef struct {
 /* num_buckets: 0 for calls without a gradient of a table. */
 LUNA_API int64_t luna_graph_softmax_scratch_bytes(int dtype, const luna_row_table* rows, int64_t heads, int64_t num_buckets);
 LUNA_API int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, const void* logits, const void* table,
-                                    const int32_t* buckets, const uint8_t* mask, void* alpha, int64_t heads,
+                                    const int32_t* buckets, const uint8_t* mask, void* alpha, void* wide, int64_t heads,
                                     int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream);
 LUNA_API int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g,
                                     const int32_t* buckets, void* glogits, void* gtable, int64_t heads, int64_t num_buckets,

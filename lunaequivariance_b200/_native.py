@@ -144,7 +144,7 @@ _SIGNATURES = {
     "luna_relative_bias_scratch_bytes": (ctypes.c_int64, [ctypes.c_int, *[ctypes.c_int64] * 3]),
     "luna_relative_bias_bwd": (ctypes.c_int, [ctypes.c_int, *[_P] * 4, *[ctypes.c_int64] * 4, _P]),
     "luna_graph_softmax_scratch_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.POINTER(RowTable), *[ctypes.c_int64] * 2]),
-    "luna_graph_softmax_fwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
+    "luna_graph_softmax_fwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 6, *[ctypes.c_int64] * 2, _P,
                                               ctypes.c_int64, _P]),
     "luna_graph_softmax_bwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
                                               ctypes.c_int64, _P]),

@@ -37,10 +37,24 @@ int pointer(const Call& c, const void* p, const char* name, bool required) {
   return aligned_to(p, rows::size_of(c.dtype)) ? LUNA_OK : fail(LUNA_ERR_MISALIGNED, "%s is not aligned to its element size", name);
 }
 
+// In the type that sums are held in, whole packets of 16 bytes.
+int wide_pointer(const Call& c, const void* p, const char* name, bool required) {
+  if (!p) return required ? fail(LUNA_ERR_INVALID_ARGUMENT, "%s is null", name) : LUNA_OK;
+  return aligned_to(p, c.dtype == LUNA_BF16 || c.dtype == LUNA_F16 ? 16 : rows::acc_size_of(c.dtype))
+             ? LUNA_OK : fail(LUNA_ERR_MISALIGNED, "%s is not aligned to 16 bytes", name);
+}
+
 // Room for the sums of the pieces, rounded up, so that what follows it is aligned.
 int64_t pieces_bytes(const Call& c) {
   return ceil_div(c.table->num_pieces * c.heads * 2 * rows::acc_size_of(c.dtype), 16) * 16;
 }
+
+// 16-bit types: room for the logits' gradient as it is before it is rounded, of which the table's is made.
+int64_t unrounded_bytes(const Call& c) {
+  return c.dtype == LUNA_BF16 || c.dtype == LUNA_F16 ? ceil_div(c.table->num_edges * c.heads * 4, 16) * 16 : 0;
+}
+// The type that the table's gradient is summed from.
+int summed_dtype(int dtype) { return dtype == LUNA_BF16 || dtype == LUNA_F16 ? LUNA_F32 : dtype; }
 
 int scratch_fits(int64_t needed, const void* scratch, int64_t bytes) {
   if (!needed) return LUNA_OK;
@@ -63,16 +77,16 @@ extern "C" int64_t luna_graph_softmax_scratch_bytes(int dtype, const luna_row_ta
   if (const int status = luna::softmax::describe(call, &R)) return status;
   int64_t bytes = luna::softmax::pieces_bytes(call);
   if (num_buckets > 0) {
-    const int64_t more = luna_relative_bias_scratch_bytes(dtype, rows->num_edges, num_buckets, heads);
+    const int64_t more = luna_relative_bias_scratch_bytes(luna::softmax::summed_dtype(dtype), rows->num_edges, num_buckets, heads);
     if (more < 0) return more;
-    bytes += more;
+    bytes += more + luna::softmax::unrounded_bytes(call);
   }
   return bytes;
 }
 
 extern "C" int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, const void* logits, const void* table,
-                                      const int32_t* buckets, const uint8_t* mask, void* alpha, int64_t heads, int64_t num_buckets,
-                                      void* scratch, int64_t scratch_bytes, void* stream) {
+                                      const int32_t* buckets, const uint8_t* mask, void* alpha, void* wide, int64_t heads,
+                                      int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
   const Call call{dtype, rows, heads, num_buckets};
@@ -83,6 +97,7 @@ extern "C" int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, con
   if ((status = softmax::pointer(call, logits, "logits", any))) return status;
   if ((status = softmax::pointer(call, alpha, "alpha", any))) return status;
   if ((status = softmax::pointer(call, table, "table", false))) return status;
+  if ((status = softmax::wide_pointer(call, wide, "wide", false))) return status;
   if (table && any && (!buckets || num_buckets < 1)) return fail(LUNA_ERR_INVALID_ARGUMENT, "a table needs buckets");
   if ((status = softmax::scratch_fits(softmax::pieces_bytes(call), scratch, scratch_bytes))) return status;
   if (!any) return LUNA_OK;
@@ -94,6 +109,7 @@ extern "C" int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, con
     o.buckets = buckets;
     o.mask = mask;
     o.out = static_cast<T*>(alpha);
+    o.wide = sizeof(T) == 2 ? static_cast<rows::Acc<T>*>(wide) : nullptr;
     status = softmax::run<T>(softmax::kForward, bias::packet_of(sizeof(T), heads, {logits, table, alpha}), R, rows->num_edges, heads,
                              num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
   });
@@ -110,32 +126,42 @@ extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, con
   int status = softmax::describe(call, &R);
   if (status) return status;
   const bool any = rows->num_edges > 0;
-  if ((status = softmax::pointer(call, alpha, "alpha", any))) return status;
+  if ((status = softmax::wide_pointer(call, alpha, "alpha", any))) return status;
   if ((status = softmax::pointer(call, g, "g", any))) return status;
   if ((status = softmax::pointer(call, glogits, "glogits", any))) return status;
   if ((status = softmax::pointer(call, gtable, "gtable", false))) return status;
   if (gtable && ((any && !buckets) || num_buckets < 1)) return fail(LUNA_ERR_INVALID_ARGUMENT, "a table needs buckets");
-  const int64_t pieces = softmax::pieces_bytes(call);
-  int64_t needed = pieces, sums = 0;
+  const int64_t pieces = softmax::pieces_bytes(call), unrounded = gtable ? softmax::unrounded_bytes(call) : 0;
+  int64_t sums = 0;
   if (gtable) {
-    sums = luna_relative_bias_scratch_bytes(dtype, rows->num_edges, num_buckets, heads);
+    sums = luna_relative_bias_scratch_bytes(softmax::summed_dtype(dtype), rows->num_edges, num_buckets, heads);
     if (sums < 0) return static_cast<int>(sums);
-    needed += sums;
   }
-  if ((status = softmax::scratch_fits(needed, scratch, scratch_bytes))) return status;
+  if ((status = softmax::scratch_fits(pieces + unrounded + sums, scratch, scratch_bytes))) return status;
+  auto* const room = static_cast<unsigned char*>(scratch);
+  void* const wide = unrounded ? room + pieces : nullptr;
   if (any)
     rows::with_type(dtype, [&](auto zero) {
       using T = decltype(zero);
       softmax::Operands<T> o{};
-      o.alpha = static_cast<const T*>(alpha);
+      o.alpha = static_cast<const rows::Acc<T>*>(alpha);
       o.g = static_cast<const T*>(g);
       o.out = static_cast<T*>(glogits);
-      status = softmax::run<T>(softmax::kBackward, bias::packet_of(sizeof(T), heads, {alpha, g, glogits}), R, rows->num_edges, heads,
-                               num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
+      o.wide = static_cast<rows::Acc<T>*>(wide);
+      const int vec = sizeof(T) == 2 ? bias::packet_of(sizeof(T), heads, {g, glogits}) : bias::packet_of(sizeof(T), heads, {alpha, g, glogits});
+      status = softmax::run<T>(softmax::kBackward, vec, R, rows->num_edges, heads, num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
     });
   if (status || !gtable) return status;
-  return luna_relative_bias_bwd(dtype, glogits, buckets, gtable, static_cast<unsigned char*>(scratch) + pieces, sums, rows->num_edges,
-                                num_buckets, heads, stream);
+  rows::with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const auto on = static_cast<cudaStream_t>(stream);
+    void* const parts = room + pieces + unrounded;
+    if constexpr (sizeof(T) == 2)
+      status = bias::table_gradient<float, T>(wide, buckets, gtable, parts, rows->num_edges, num_buckets, heads, on);
+    else
+      status = bias::table_gradient<T, T>(glogits, buckets, gtable, parts, rows->num_edges, num_buckets, heads, on);
+  });
+  return status;
 }
 
 extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
@@ -148,7 +174,7 @@ extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows,
   int status = softmax::describe(call, &R);
   if (status) return status;
   const bool any = rows->num_edges > 0;
-  if ((status = softmax::pointer(call, alpha, "alpha", any))) return status;
+  if ((status = softmax::wide_pointer(call, alpha, "alpha", any))) return status;
   if ((status = softmax::pointer(call, g, "g", any))) return status;
   if ((status = softmax::pointer(call, r, "r", false))) return status;
   if ((status = softmax::pointer(call, rtable, "rtable", false))) return status;
@@ -160,15 +186,16 @@ extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows,
   rows::with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     softmax::Operands<T> o{};
-    o.alpha = static_cast<const T*>(alpha);
+    o.alpha = static_cast<const rows::Acc<T>*>(alpha);
     o.g = static_cast<const T*>(g);
     o.r = static_cast<const T*>(r);
     o.rtable = static_cast<const T*>(rtable);
     o.buckets = buckets;
     o.out = static_cast<T*>(hg);
     o.out2 = static_cast<T*>(halpha);
-    status = softmax::run<T>(softmax::kSecond, bias::packet_of(sizeof(T), heads, {alpha, g, r, rtable, halpha, hg}), R, rows->num_edges,
-                             heads, num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
+    const int vec = sizeof(T) == 2 ? bias::packet_of(sizeof(T), heads, {g, r, rtable, halpha, hg})
+                                   : bias::packet_of(sizeof(T), heads, {alpha, g, r, rtable, halpha, hg});
+    status = softmax::run<T>(softmax::kSecond, vec, R, rows->num_edges, heads, num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
   });
   return status;
 }

@@ -14,6 +14,8 @@
 // pieces, one joins those of each cut node, and one makes the pieces' outputs.
 #pragma once
 
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace luna {
@@ -39,10 +41,13 @@ enum Phase { kWhole, kMixed, kApply };  // no pieces; whole rows and the pieces'
 
 template <typename T>
 struct Operands {
-  const T *logits, *table, *alpha, *g, *r, *rtable;
+  const T *logits, *table;
+  const Acc<T>* alpha;  // as the sums are held: rounded to 16 bits, the sums by bucket of alpha (g - D) are off by more than their own rounding
+  const T *g, *r, *rtable;
   const int32_t* buckets;
   const uint8_t* mask;
   T *out, *out2;
+  Acc<T>* wide;  // 16-bit types: the output once more, as it was before it was rounded
 };
 
 template <typename A>
@@ -147,12 +152,12 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
   auto fetch = [&](int first, int left) {
     const int64_t at = static_cast<int64_t>(first) * S.heads + head;
     auto there = [&](int k) { return k * slots < left; };
-    auto bring = [&](const T* __restrict__ array, A (&to)[K][VEC], A otherwise) {
-      const T* from = array + at;
+    auto bring = [&](const auto* __restrict__ array, A (&to)[K][VEC], A otherwise) {
+      const auto* from = array + at;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (there(k)) {
-          rows::load<T, VEC>(from + k * stride, to[k]);
+          rows::load<std::remove_const_t<std::remove_pointer_t<decltype(from)>>, VEC>(from + k * stride, to[k]);
         } else {
 #pragma unroll
           for (int c = 0; c < VEC; ++c) to[k][c] = otherwise;
@@ -231,6 +236,8 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
         }
       }
       if (ORDER != kSecond || o.out) rows::store<T, VEC>(out + k * stride, v);
+      if constexpr (sizeof(T) == 2 && ORDER != kSecond)
+        if (o.wide) rows::store<A, VEC>(o.wide + at + k * stride, v);
       if constexpr (ORDER == kSecond)
         if (o.out2) rows::store<T, VEC>(out2 + k * stride, w);
     }

@@ -164,7 +164,7 @@ extern "C" int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* b
                 static_cast<long long>(scratch ? scratch_bytes : 0));
   if (!aligned_to(scratch, 16)) return fail(LUNA_ERR_MISALIGNED, "scratch is not aligned to 16 bytes");
   rows::with_type(dtype, [&](auto zero) {
-    status = bias::table_gradient<decltype(zero)>(g, buckets, gtable, scratch, edges, num_buckets, heads, static_cast<cudaStream_t>(stream));
+    status = bias::table_gradient<decltype(zero), decltype(zero)>(g, buckets, gtable, scratch, edges, num_buckets, heads, static_cast<cudaStream_t>(stream));
   });
   return status;
 }

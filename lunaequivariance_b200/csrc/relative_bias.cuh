@@ -226,8 +226,9 @@ inline int64_t partial_numbers(int64_t size, int64_t acc_size, int64_t edges, in
   return parts * num_buckets * heads;
 }
 
-template <typename T, int VEC>
-int table_gradient(const T* g, const int32_t* buckets, T* gtable, void* scratch, int64_t edges, int64_t num_buckets, int64_t heads,
+// TO: the type of the table, if it is narrower than its gradient's parts.
+template <typename T, typename TO, int VEC>
+int table_gradient(const T* g, const int32_t* buckets, TO* gtable, void* scratch, int64_t edges, int64_t num_buckets, int64_t heads,
                    cudaStream_t stream) {
   using A = Acc<T>;
   const Cut cut = cut_of(sizeof(A), VEC, edges, num_buckets, heads);
@@ -244,25 +245,25 @@ int table_gradient(const T* g, const int32_t* buckets, T* gtable, void* scratch,
       g, buckets, partial, edges, static_cast<int>(num_buckets), static_cast<int>(heads), cut, aligned_to(buckets, 16));
   LUNA_LAUNCH_CHECK("gradient of the bias table");
   const int64_t numbers = num_buckets * heads;
-  launch_early(table_final_kernel<T>, dim3(static_cast<unsigned>(ceil_div(numbers, 32))), 32 * kFinalSlices, 0, stream,
+  launch_early(table_final_kernel<TO>, dim3(static_cast<unsigned>(ceil_div(numbers, 32))), 32 * kFinalSlices, 0, stream,
                static_cast<const A*>(partial), gtable, numbers, cut.parts_of_edges);
   LUNA_LAUNCH_CHECK("sums of the bias table");
   return LUNA_OK;
 }
 
-template <typename T>
+template <typename T, typename TO>
 int table_gradient(const void* g_, const int32_t* buckets, void* gtable_, void* scratch, int64_t edges, int64_t num_buckets,
                    int64_t heads, cudaStream_t stream) {
   const T* g = static_cast<const T*>(g_);
-  T* gtable = static_cast<T*>(gtable_);
+  TO* gtable = static_cast<TO*>(gtable_);
   switch (packet_of(sizeof(T), heads, {g})) {
-    case 1: return table_gradient<T, 1>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
-    case 2: return table_gradient<T, 2>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
+    case 1: return table_gradient<T, TO, 1>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
+    case 2: return table_gradient<T, TO, 2>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
     case 4:
-      if constexpr (sizeof(T) <= 4) return table_gradient<T, 4>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
+      if constexpr (sizeof(T) <= 4) return table_gradient<T, TO, 4>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
       break;
     case 8:
-      if constexpr (sizeof(T) <= 2) return table_gradient<T, 8>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
+      if constexpr (sizeof(T) <= 2) return table_gradient<T, TO, 8>(g, buckets, gtable, scratch, edges, num_buckets, heads, stream);
       break;
   }
   return LUNA_ERR_UNSUPPORTED;

@@ -1083,7 +1083,11 @@ void check_table(const Tensor& x, const Tensor& table, const Tensor& buckets) {
   check_beside(x, buckets, "buckets", {x.size(0)}, at::kInt);
 }
 
-Tensor softmax_forward(const Rows& rows, const Tensor& logits, const Tensor& table, const Tensor& buckets, const Tensor& mask) {
+bool narrow(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+
+// alpha, and what the backward makes gradients of: alpha itself, or for the 16-bit types alpha before it was rounded.
+std::array<Tensor, 2> softmax_forward(const Rows& rows, const Tensor& logits, const Tensor& table, const Tensor& buckets, const Tensor& mask,
+                                      bool differentiated) {
   const int dtype = check_softmax(rows, logits, "logits");
   refuse_tangents({&table});
   TORCH_CHECK_VALUE(table.defined() == buckets.defined(), "a bias table and the edges' buckets come together");
@@ -1091,17 +1095,26 @@ Tensor softmax_forward(const Rows& rows, const Tensor& logits, const Tensor& tab
   check_beside(logits, mask, "mask", {logits.size(0)}, at::kBool);
   const c10::cuda::CUDAGuard guard(logits.device());
   const Tensor z = logits.contiguous(), t = contiguous(table), b = contiguous(buckets), m = contiguous(mask);
-  Tensor alpha = at::empty(z.sizes(), z.options());
+  Tensor alpha = at::empty(z.sizes(), z.options()), wide;
+  if (differentiated && narrow(z)) wide = at::empty(z.sizes(), z.options().dtype(at::kFloat));
   const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(z), 0), z);
   check(api.softmax_fwd(dtype, &rows.native, z.data_ptr(), pointer(t), static_cast<const int32_t*>(pointer(b)),
-                        static_cast<const uint8_t*>(pointer(m)), alpha.data_ptr(), heads_of(z), t.defined() ? t.size(0) : 0,
+                        static_cast<const uint8_t*>(pointer(m)), alpha.data_ptr(), pointer(wide), heads_of(z), t.defined() ? t.size(0) : 0,
                         pointer(scratch), bytes_of(scratch), stream_of(z)));
-  return alpha;
+  return {alpha, wide};
+}
+
+// What the launches read alpha from: `wide` where there is one.  Other alphas of 16 bits are what a caller of the operators has made.
+Tensor exact_alpha(const Tensor& alpha, const Tensor& wide) {
+  if (!narrow(alpha)) return alpha.contiguous();
+  if (!wide.defined() || !wide.numel()) return alpha.to(at::kFloat).contiguous();
+  check_beside(alpha, wide, "wide", alpha.sizes(), at::kFloat);
+  return wide.contiguous();
 }
 
 // The gradients of the logits and of the table, as far as `mask` names them.
-std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, const Tensor& g, const Tensor& buckets, int64_t num_buckets,
-                                       int mask) {
+std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, const Tensor& wide, const Tensor& g, const Tensor& buckets,
+                                       int64_t num_buckets, int mask) {
   std::array<Tensor, 2> out;
   if (!mask) return out;
   const int dtype = check_softmax(rows, alpha, "alpha");
@@ -1109,19 +1122,19 @@ std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, co
   check_beside(alpha, g, "grad_out", alpha.sizes());
   check_table(alpha, Tensor(), buckets);
   const c10::cuda::CUDAGuard guard(alpha.device());
-  const Tensor a = alpha.contiguous(), e = g.contiguous(), b = contiguous(buckets);
-  out[0] = at::empty(a.sizes(), a.options());  // the table's gradient is made of it
-  if (mask & 2) out[1] = at::empty({num_buckets, heads_of(a)}, a.options());
-  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(a), mask & 2 ? num_buckets : 0), a);
+  const Tensor a = exact_alpha(alpha, wide), e = g.contiguous(), b = contiguous(buckets);
+  out[0] = at::empty(e.sizes(), e.options());  // the table's gradient is made of it
+  if (mask & 2) out[1] = at::empty({num_buckets, heads_of(e)}, e.options());
+  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(e), mask & 2 ? num_buckets : 0), e);
   check(api.softmax_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), static_cast<const int32_t*>(pointer(b)), out[0].data_ptr(),
-                        pointer(out[1]), heads_of(a), num_buckets, pointer(scratch), bytes_of(scratch), stream_of(a)));
+                        pointer(out[1]), heads_of(e), num_buckets, pointer(scratch), bytes_of(scratch), stream_of(e)));
   if (!(mask & 1)) out[0] = Tensor();
   return out;
 }
 
 // The derivatives with respect to alpha and g named in `mask`.
-std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, const Tensor& g, const Tensor& buckets, const Tensor& r,
-                                     const Tensor& rtable, int mask) {
+std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, const Tensor& wide, const Tensor& g, const Tensor& buckets,
+                                     const Tensor& r, const Tensor& rtable, int mask) {
   std::array<Tensor, 2> out;
   if (!mask) return out;
   const int dtype = check_softmax(rows, alpha, "alpha");
@@ -1130,40 +1143,40 @@ std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, cons
   check_beside(alpha, r, "r", alpha.sizes());
   check_table(alpha, rtable, buckets);
   const c10::cuda::CUDAGuard guard(alpha.device());
-  const Tensor a = alpha.contiguous(), e = g.contiguous(), b = contiguous(buckets), t = contiguous(r), tt = contiguous(rtable);
+  const Tensor a = exact_alpha(alpha, wide), e = g.contiguous(), b = contiguous(buckets), t = contiguous(r), tt = contiguous(rtable);
   for (int s = 0; s < 2; ++s)
-    if (mask >> s & 1) out[s] = at::empty(a.sizes(), a.options());
-  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(a), 0), a);
+    if (mask >> s & 1) out[s] = at::empty(e.sizes(), e.options());
+  const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(e), 0), e);
   check(api.softmax_dbl_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), pointer(t), pointer(tt), static_cast<const int32_t*>(pointer(b)),
-                            pointer(out[0]), pointer(out[1]), heads_of(a), tt.defined() ? tt.size(0) : 0, pointer(scratch), bytes_of(scratch),
-                            stream_of(a)));
+                            pointer(out[0]), pointer(out[1]), heads_of(e), tt.defined() ? tt.size(0) : 0, pointer(scratch), bytes_of(scratch),
+                            stream_of(e)));
   return out;
 }
 
 struct SoftmaxDouble : Function<SoftmaxDouble> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
-                               const Maybe& rtable, int64_t mask, const RowsPtr& rows) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& wide, const Maybe& buckets,
+                               const Maybe& r, const Maybe& rtable, int64_t mask, const RowsPtr& rows) {
     ctx->set_materialize_grads(false);
-    return only(softmax_double(*rows, alpha, g, of(buckets), of(r), of(rtable), static_cast<int>(mask)), static_cast<int>(mask));
+    return only(softmax_double(*rows, alpha, of(wide), g, of(buckets), of(r), of(rtable), static_cast<int>(mask)), static_cast<int>(mask));
   }
   static variable_list backward(AutogradContext*, const variable_list& grads) {
     for (const Tensor& t : grads)
       TORCH_CHECK_NOT_IMPLEMENTED(!t.defined(), "third-order derivatives of the softmax over in-edges are not provided");
-    return variable_list(7);
+    return variable_list(8);
   }
 };
 
 struct SoftmaxBackward : Function<SoftmaxBackward> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
-                               int64_t mask, const RowsPtr& rows) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& wide, const Maybe& buckets,
+                               int64_t num_buckets, int64_t mask, const RowsPtr& rows) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({alpha, g, of(buckets)});
+    ctx->save_for_backward({alpha, g, of(wide), of(buckets)});
     ctx->saved_data["mask"] = mask;
     keep(ctx, "rows", rows);
-    return only(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, static_cast<int>(mask)), static_cast<int>(mask));
+    return only(softmax_backward(*rows, alpha, of(wide), g, of(buckets), num_buckets, static_cast<int>(mask)), static_cast<int>(mask));
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    variable_list out(6);
+    variable_list out(7);
     const auto r = spread<2>(grads, static_cast<int>(ctx->saved_data["mask"].toInt()));
     if (!r[0].defined() && !r[1].defined()) return out;
     const auto saved = ctx->get_saved_variables();
@@ -1171,9 +1184,9 @@ struct SoftmaxBackward : Function<SoftmaxBackward> {
     if (!mask) return out;
     const auto rows = kept<Rows>(ctx, "rows");
     const auto h = at::GradMode::is_enabled()
-                       ? spread<2>(SoftmaxDouble::apply(saved[0], saved[1], maybe(saved[2]), maybe(r[0]), maybe(r[1]),
+                       ? spread<2>(SoftmaxDouble::apply(saved[0], saved[1], maybe(saved[2]), maybe(saved[3]), maybe(r[0]), maybe(r[1]),
                                                         static_cast<int64_t>(mask), rows), mask)
-                       : softmax_double(*rows, saved[0], saved[1], saved[2], r[0], r[1], mask);
+                       : softmax_double(*rows, saved[0], saved[2], saved[1], saved[3], r[0], r[1], mask);
     for (int s = 0; s < 2; ++s) out[s] = h[s];
     return out;
   }
@@ -1182,12 +1195,12 @@ struct SoftmaxBackward : Function<SoftmaxBackward> {
 struct SoftmaxForward : Function<SoftmaxForward> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask,
                         const RowsPtr& rows) {
-    const Tensor alpha = softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+    const auto found = softmax_forward(*rows, logits, of(table), of(buckets), of(mask), true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({alpha, of(buckets)});  // alpha says all about the logits, the table and the mask
+    ctx->save_for_backward({found[0], found[1], of(buckets)});  // alpha says all about the logits, the table and the mask
     ctx->saved_data["buckets"] = table ? table->size(0) : 0;
     keep(ctx, "rows", rows);
-    return alpha;
+    return found[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(5);
@@ -1199,8 +1212,9 @@ struct SoftmaxForward : Function<SoftmaxForward> {
     if (!mask) return out;
     const auto rows = kept<Rows>(ctx, "rows");
     const auto d = at::GradMode::is_enabled()
-                       ? spread<2>(SoftmaxBackward::apply(saved[0], grads[0], maybe(saved[1]), num_buckets, static_cast<int64_t>(mask), rows), mask)
-                       : softmax_backward(*rows, saved[0], grads[0], saved[1], num_buckets, mask);
+                       ? spread<2>(SoftmaxBackward::apply(saved[0], grads[0], maybe(saved[1]), maybe(saved[2]), num_buckets,
+                                                          static_cast<int64_t>(mask), rows), mask)
+                       : softmax_backward(*rows, saved[0], saved[1], grads[0], saved[2], num_buckets, mask);
     for (int s = 0; s < 2; ++s) out[s] = d[s];
     return out;
   }
@@ -1209,7 +1223,7 @@ struct SoftmaxForward : Function<SoftmaxForward> {
 Tensor graph_softmax(const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
   pybind11::gil_scoped_release release;
   return tracked({&logits, &of(table)}) ? SoftmaxForward::apply(logits, table, buckets, mask, rows)
-                                        : softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+                                        : softmax_forward(*rows, logits, of(table), of(buckets), of(mask), false)[0];
 }
 
 // The launches alone, for the operators that a traced program names.
@@ -1249,13 +1263,16 @@ PYBIND11_MODULE(luna_torch, m) {
   }));
   m.def("relative_bias_forward", torch::wrap_pybind_function(bias_forward));
   m.def("relative_bias_backward", torch::wrap_pybind_function(bias_backward));
-  m.def("graph_softmax_forward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
-    return softmax_forward(*rows, logits, of(table), of(buckets), of(mask));
+  m.def("graph_softmax_forward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& logits, const Maybe& table,
+                                                                const Maybe& buckets, const Maybe& mask) {
+    return listed(softmax_forward(*rows, logits, of(table), of(buckets), of(mask), true));
   }));
-  m.def("graph_softmax_backward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
-                                     int mask) { return listed(softmax_backward(*rows, alpha, g, of(buckets), num_buckets, mask)); }));
-  m.def("graph_softmax_double", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
-                                   const Maybe& rtable, int mask) {
-    return listed(softmax_double(*rows, alpha, g, of(buckets), of(r), of(rtable), mask));
+  m.def("graph_softmax_backward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Maybe& wide, const Tensor& g,
+                                                                 const Maybe& buckets, int64_t num_buckets, int mask) {
+    return listed(softmax_backward(*rows, alpha, of(wide), g, of(buckets), num_buckets, mask));
+  }));
+  m.def("graph_softmax_double", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Maybe& wide, const Tensor& g,
+                                                               const Maybe& buckets, const Maybe& r, const Maybe& rtable, int mask) {
+    return listed(softmax_double(*rows, alpha, of(wide), g, of(buckets), of(r), of(rtable), mask));
   }));
 }

@@ -26,72 +26,79 @@ def _rows(rowptr, edges):
     return _native.binding().Rows(rowptr, edges, None, None, None, None)
 
 
-@torch.library.custom_op("lunaeq::graph_softmax_forward", mutates_args=())
-def graph_softmax_forward_op(logits: torch.Tensor, table: torch.Tensor | None, buckets: torch.Tensor | None,
-                             mask: torch.Tensor | None, rowptr: torch.Tensor, edges: int) -> torch.Tensor:
-    return _native.binding().graph_softmax_forward(_rows(rowptr, edges), logits, table, buckets, mask)
+@torch.library.custom_op("lunaeq::graph_softmax_forward", mutates_args=(),
+                         schema="(Tensor logits, Tensor? table, Tensor? buckets, Tensor? mask, Tensor rowptr, SymInt edges)"
+                                " -> (Tensor, Tensor)")
+def graph_softmax_forward_op(logits, table, buckets, mask, rowptr, edges):
+    """The result, and for 16-bit types the result before it was rounded (else nothing)."""
+    alpha, wide = _native.binding().graph_softmax_forward(_rows(rowptr, edges), logits, table, buckets, mask)
+    return alpha, logits.new_empty(0, dtype=torch.float32) if wide is None else wide
 
 
 @graph_softmax_forward_op.register_fake
 def _(logits, table, buckets, mask, rowptr, edges):
-    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+    alpha = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    narrow = logits.dtype in (torch.bfloat16, torch.float16)
+    return alpha, alpha.new_empty(alpha.shape if narrow else (0,), dtype=torch.float32)
 
 
 @torch.library.custom_op("lunaeq::graph_softmax_backward", mutates_args=(),
-                         schema="(Tensor alpha, Tensor g, Tensor? buckets, SymInt num_buckets, Tensor rowptr, bool[] needs)"
-                                " -> (Tensor?, Tensor?)")
-def graph_softmax_backward_op(alpha, g, buckets, num_buckets, rowptr, needs):
-    return tuple(_native.binding().graph_softmax_backward(_rows(rowptr, alpha.shape[0]), alpha, g, buckets, num_buckets,
-                                                          _mask(needs)))
+                         schema="(Tensor alpha, Tensor wide, Tensor g, Tensor? buckets, SymInt num_buckets, Tensor rowptr,"
+                                " bool[] needs) -> (Tensor?, Tensor?)")
+def graph_softmax_backward_op(alpha, wide, g, buckets, num_buckets, rowptr, needs):
+    return tuple(_native.binding().graph_softmax_backward(_rows(rowptr, alpha.shape[0]), alpha, wide, g, buckets,
+                                                          num_buckets, _mask(needs)))
 
 
 @graph_softmax_backward_op.register_fake
-def _(alpha, g, buckets, num_buckets, rowptr, needs):
+def _(alpha, wide, g, buckets, num_buckets, rowptr, needs):
     heads = alpha.shape[1] if alpha.ndim == 2 else 1
     return (torch.empty_like(alpha, memory_format=torch.contiguous_format) if needs[0] else None,
             alpha.new_empty((num_buckets, heads)) if needs[1] else None)
 
 
 @torch.library.custom_op("lunaeq::graph_softmax_double_backward", mutates_args=(),
-                         schema="(Tensor alpha, Tensor g, Tensor? buckets, Tensor? r, Tensor? rtable, Tensor rowptr,"
+                         schema="(Tensor alpha, Tensor wide, Tensor g, Tensor? buckets, Tensor? r, Tensor? rtable, Tensor rowptr,"
                                 " bool[] needs) -> (Tensor?, Tensor?)")
-def graph_softmax_double_backward_op(alpha, g, buckets, r, rtable, rowptr, needs):
-    return tuple(_native.binding().graph_softmax_double(_rows(rowptr, alpha.shape[0]), alpha, g, buckets, r, rtable,
+def graph_softmax_double_backward_op(alpha, wide, g, buckets, r, rtable, rowptr, needs):
+    return tuple(_native.binding().graph_softmax_double(_rows(rowptr, alpha.shape[0]), alpha, wide, g, buckets, r, rtable,
                                                         _mask(needs)))
 
 
 @graph_softmax_double_backward_op.register_fake
-def _(alpha, g, buckets, r, rtable, rowptr, needs):
+def _(alpha, wide, g, buckets, r, rtable, rowptr, needs):
     return tuple(torch.empty_like(alpha, memory_format=torch.contiguous_format) if need else None for need in needs)
 
 
 def _forward_setup(ctx, inputs, output):
     _, table, buckets, _, rowptr, _ = inputs
     ctx.num_buckets = 0 if table is None else table.shape[0]
-    ctx.save_for_backward(output, buckets, rowptr)
+    ctx.save_for_backward(*output, buckets, rowptr)
+    ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)
 
 
-def _forward_backward(ctx, g):
+def _forward_backward(ctx, g, _):
     if g is None:
         return (None,) * 6
-    alpha, buckets, rowptr = ctx.saved_tensors
+    alpha, wide, buckets, rowptr = ctx.saved_tensors
     needs = [ctx.needs_input_grad[0], bool(ctx.num_buckets) and ctx.needs_input_grad[1]]
-    return (*graph_softmax_backward_op(alpha, g, buckets, ctx.num_buckets, rowptr, needs), None, None, None, None)
+    return (*graph_softmax_backward_op(alpha, wide, g, buckets, ctx.num_buckets, rowptr, needs), None, None, None, None)
 
 
 def _backward_setup(ctx, inputs, output):
-    alpha, g, buckets, _, rowptr, _ = inputs
-    ctx.save_for_backward(alpha, g, buckets, rowptr)
+    alpha, wide, g, buckets, _, rowptr, _ = inputs
+    ctx.save_for_backward(alpha, wide, g, buckets, rowptr)
     ctx.set_materialize_grads(False)
 
 
 def _backward_backward(ctx, r, rtable):
     if r is None and rtable is None:
-        return (None,) * 6
-    alpha, g, buckets, rowptr = ctx.saved_tensors
-    return (*graph_softmax_double_backward_op(alpha, g, buckets, r, rtable, rowptr, list(ctx.needs_input_grad[:2])),
-            None, None, None, None)
+        return (None,) * 7
+    alpha, wide, g, buckets, rowptr = ctx.saved_tensors
+    needs = [ctx.needs_input_grad[0], ctx.needs_input_grad[2]]
+    halpha, hg = graph_softmax_double_backward_op(alpha, wide, g, buckets, r, rtable, rowptr, needs)
+    return halpha, None, hg, None, None, None, None
 
 
 graph_softmax_forward_op.register_autograd(_forward_backward, setup_context=_forward_setup)
@@ -114,7 +121,7 @@ def graph_softmax(logits, graph, *, mask=None, table=None, buckets=None):
         raise TypeError("a bias table and the edges' buckets come together")
     if is_compiling():
         return torch.ops.lunaeq.graph_softmax_forward.default(logits, table, buckets, mask, graph.dst_rowptr,
-                                                              graph.num_edges)
+                                                              graph.num_edges)[0]
     if not logits.is_cuda:
         raise RuntimeError("CUDA is required for the softmax over in-edges in this library")
     if graph.src.device != logits.device and graph.num_edges:

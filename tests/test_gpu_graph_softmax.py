@@ -136,6 +136,24 @@ def test_rows_that_must_stay_whole():
         assert torch.allclose(luna.graph_softmax(logits.to(DEVICE), whole).cpu(), want, rtol=1e-12, atol=0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_sums_by_bucket_are_not_made_of_rounded_parts(dtype):
+    """Almost all edges of a row in one bucket: its gradient is what is left of sums that cancel, as exact as its own rounding."""
+    generator = torch.Generator().manual_seed(3)
+    graph, dst = graph_of([50] * 200, generator)
+    buckets = (torch.rand(10_000, generator=generator) < 0.05).to(torch.int32)
+    z, g = ((2 * torch.randn(10_000, 4, generator=generator, dtype=F64)).to(dtype) for _ in range(2))
+    table = torch.randn(2, 4, generator=generator, dtype=F64).to(dtype)
+    leaf = table.to(DEVICE).requires_grad_(True)
+    got, = torch.autograd.grad(luna.graph_softmax(z.to(DEVICE), graph, table=leaf, buckets=buckets.to(DEVICE)), leaf, g.to(DEVICE))
+    reference = table.double().requires_grad_(True)
+    alpha = oracle.graph_softmax(z.double(), dst, 200, table=reference, buckets=buckets)
+    want, = torch.autograd.grad(alpha, reference, g.double())
+    # the rounding of the result, and 200 roundings in single precision of what is added up: alpha times twice the largest g
+    allowed = step(dtype) * want.abs() + 200 * step(F32) * (alpha.detach() * 2 * g.double().abs().max()).sum(0)
+    assert ((got.cpu().double() - want).abs() <= allowed).all()
+
+
 def test_gradient_against_differences():
     for kind, buckets in (("mixed", 0), ("small", 6)):
         graph, _, _, p = problem(kind, 2, buckets, 0.2, F64)
@@ -268,10 +286,11 @@ def test_streams_and_captured_graphs(kind):
         assert all(torch.equal(found[k], want[k]) for k in want)
 
 
-def test_custom_ops():
-    graph, _, _, p = problem("small", 3, 6, 0.2, F64)
+@pytest.mark.parametrize("dtype", [F64, BF16])
+def test_custom_ops(dtype):
+    graph, _, _, p = problem("small", 3, 6, 0.2, dtype)
     p = {k: None if v is None else v.to(DEVICE) for k, v in p.items()}
-    ops = lambda z, t: torch.ops.lunaeq.graph_softmax_forward(z, t, p["buckets"], p["mask"], graph.dst_rowptr, graph.num_edges)  # noqa: E731
+    ops = lambda z, t: torch.ops.lunaeq.graph_softmax_forward(z, t, p["buckets"], p["mask"], graph.dst_rowptr, graph.num_edges)[0]  # noqa: E731
     own = lambda z, t: luna.graph_softmax(z, graph, mask=p["mask"], table=t, buckets=p["buckets"])  # noqa: E731
     want, got = derivatives(own, p), derivatives(ops, p)
     assert all(torch.equal(got[k], want[k]) for k in want)

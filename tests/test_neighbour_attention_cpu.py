@@ -82,7 +82,7 @@ def test_descriptions_are_checked_at_the_entry_points():
     assert lib.luna_distance_buckets(2, some, some, 1, some, 1, None) == _native.LUNA_ERR_INVALID_ARGUMENT
     table = _native.RowTable(2, 4, 0, 0, 16)
     softmax = lambda t, **k: lib.luna_graph_softmax_fwd(  # noqa: E731
-        k.get("dtype", 0), ctypes.byref(t), k.get("logits", some), k.get("table"), None, None, some, k.get("heads", 1), 0, None, 0, None)
+        k.get("dtype", 0), ctypes.byref(t), k.get("logits", some), k.get("table"), None, None, some, None, k.get("heads", 1), 0, None, 0, None)
     assert softmax(table, heads=0) == softmax(table, dtype=9) == softmax(table, logits=None) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert softmax(table, table=some) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert softmax(_native.RowTable(2, 4, 0, 0, None)) == _native.LUNA_ERR_INVALID_ARGUMENT
