@@ -65,7 +65,9 @@ template <typename T, int VEC>
 void gather(const T* table, const int32_t* buckets, T* out, int64_t edges, int64_t num_buckets, int64_t heads, cudaStream_t stream) {
   const int64_t packets = heads / VEC;
   const int lanes = packets >= 32 ? 32 : rows::next_power_of_two(packets);
-  const int64_t ctas = ceil_div(edges, 256 / lanes), most = static_cast<int64_t>(rows::processors()) * 64;
+  // Short rows: the CTAs that are resident go from edge to edge (2 M edges of 8 floats, 8 or 128 CTAs a multiprocessor, 12 and 17 us);
+  // long ones are handed out by the hardware (209,000 of 704 floats 100 and 84).
+  const int64_t ctas = ceil_div(edges, 256 / lanes), most = static_cast<int64_t>(rows::processors()) * (lanes < 32 ? 8 : 128);
   gather_kernel<T, VEC><<<static_cast<unsigned>(ctas < most ? ctas : most), 256, 0, stream>>>(
       table, buckets, out, edges, static_cast<int>(num_buckets), static_cast<int>(heads), lanes);
 }
@@ -99,7 +101,7 @@ extern "C" int luna_distance_buckets(int dtype, const void* vec, const void* bou
   if (!status) status = bias::check_pointer(size, boundaries, "boundaries", num_boundaries > 0);
   if (!status) status = bias::check_pointer(4, out, "out", n > 0);
   if (status || n == 0) return status;
-  const int64_t ctas = ceil_div(n, 1024), most = static_cast<int64_t>(rows::processors()) * 16;
+  const int64_t ctas = ceil_div(n, 1024), most = static_cast<int64_t>(rows::processors()) * 8;
   const bool aligned = aligned_to(vec, 16) && aligned_to(out, 16);
   const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
   const int count = static_cast<int>(num_boundaries);
