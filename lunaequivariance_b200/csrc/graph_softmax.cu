@@ -10,6 +10,7 @@ struct Call {
   int dtype;
   const luna_row_table* table;
   int64_t heads, num_buckets;
+  const int32_t* buckets;
 };
 
 int describe(const Call& c, Rows* R) {
@@ -28,6 +29,8 @@ int describe(const Call& c, Rows* R) {
     return fail(LUNA_ERR_INVALID_ARGUMENT, "pieces that no rows have");
   if (t.num_pieces > 0 && (!t.piece_of_row || !t.row_of_piece || !t.cut_of_piece || !t.cut_first))
     return fail(LUNA_ERR_INVALID_ARGUMENT, "tables of the pieces missing");
+  for (const int32_t* p : {t.rowptr, t.piece_of_row, t.row_of_piece, t.cut_of_piece, t.cut_first, c.buckets})
+    if (!aligned_to(p, 4)) return fail(LUNA_ERR_MISALIGNED, "a table of 32-bit indices is not aligned to them");
   *R = Rows{t.rowptr, t.num_rows, t.num_pieces, t.num_cut, t.piece_of_row, t.row_of_piece, t.cut_of_piece, t.cut_first};
   return LUNA_OK;
 }
@@ -72,7 +75,7 @@ using luna::softmax::Call;
 
 extern "C" int64_t luna_graph_softmax_scratch_bytes(int dtype, const luna_row_table* rows, int64_t heads, int64_t num_buckets) {
   luna::clear_error();
-  const Call call{dtype, rows, heads, num_buckets};
+  const Call call{dtype, rows, heads, num_buckets, nullptr};
   luna::softmax::Rows R;
   if (const int status = luna::softmax::describe(call, &R)) return status;
   int64_t bytes = luna::softmax::pieces_bytes(call);
@@ -89,7 +92,7 @@ extern "C" int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, con
                                       int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
-  const Call call{dtype, rows, heads, num_buckets};
+  const Call call{dtype, rows, heads, num_buckets, buckets};
   softmax::Rows R;
   int status = softmax::describe(call, &R);
   if (status) return status;
@@ -121,7 +124,7 @@ extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, con
                                       int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
-  const Call call{dtype, rows, heads, num_buckets};
+  const Call call{dtype, rows, heads, num_buckets, buckets};
   softmax::Rows R;
   int status = softmax::describe(call, &R);
   if (status) return status;
@@ -169,7 +172,7 @@ extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows,
                                           int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
-  const Call call{dtype, rows, heads, num_buckets};
+  const Call call{dtype, rows, heads, num_buckets, buckets};
   softmax::Rows R;
   int status = softmax::describe(call, &R);
   if (status) return status;

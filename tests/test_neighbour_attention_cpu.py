@@ -85,6 +85,7 @@ def test_descriptions_are_checked_at_the_entry_points():
         k.get("dtype", 0), ctypes.byref(t), k.get("logits", some), k.get("table"), None, None, some, None, k.get("heads", 1), 0, None, 0, None)
     assert softmax(table, heads=0) == softmax(table, dtype=9) == softmax(table, logits=None) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert softmax(table, table=some) == _native.LUNA_ERR_INVALID_ARGUMENT
+    assert softmax(_native.RowTable(2, 4, 0, 0, 18)) == _native.LUNA_ERR_MISALIGNED
     assert softmax(_native.RowTable(2, 4, 0, 0, None)) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert softmax(_native.RowTable(2, 1 << 31, 0, 0, 16)) == _native.LUNA_ERR_OVERFLOW
     assert softmax(_native.RowTable(2, 4, 2, 1, 16, 16, 16)) == _native.LUNA_ERR_INVALID_ARGUMENT
