@@ -83,7 +83,10 @@ table_kernel(const T* __restrict__ g, const int32_t* __restrict__ buckets, Acc<T
     if (number < count && at + AHEAD <= edges) {
       if (wide_buckets) {
 #pragma unroll
-        for (int j = 0; j < AHEAD; j += 4) *reinterpret_cast<int4*>(&to.row[j]) = *reinterpret_cast<const int4*>(bucket_at + j);
+        for (int j = 0; j < AHEAD; j += 4) {
+          const int4 four = *reinterpret_cast<const int4*>(bucket_at + j);
+          to.row[j] = four.x, to.row[j + 1] = four.y, to.row[j + 2] = four.z, to.row[j + 3] = four.w;
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) to.row[j] = bucket_at[j];
