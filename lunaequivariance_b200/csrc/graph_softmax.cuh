@@ -241,6 +241,23 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
       if constexpr (ORDER == kSecond)
         if (o.out2) rows::store<T, VEC>(out2 + k * stride, w);
     }
+    if constexpr (ORDER == kForward) {
+      // Zero times a sum that is no number is none either: what is masked beside one is put right, a walk that no other row takes.
+      // (A bit for each masked number in a register instead: 2.6 M edges with one head, mask and table 33 us, 27 like this.)
+      bool lost = false;
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) lost |= b[c] != b[c];
+      if (lost && o.mask) {
+        const A zeros[VEC] = {};
+#pragma unroll 1
+        for (int k = 0; k < K; ++k) {
+          if (k * slots >= left || o.mask[first + k * slots]) continue;
+          rows::store<T, VEC>(out + k * stride, zeros);
+          if constexpr (sizeof(T) == 2)
+            if (o.wide) rows::store<A, VEC>(o.wide + at + k * stride, zeros);
+        }
+      }
+    }
   };
   auto exponentials = [&](const A (&m)[VEC]) {
 #pragma unroll
