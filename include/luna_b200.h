@@ -308,7 +308,11 @@ LUNA_API int luna_relative_bias_bwd(int dtype, const void* g, const int32_t* buc
  * backward: glogits = alpha (g - sum alpha g), and gtable its sums by bucket (null: not wanted).  Where alpha is zero the
  *           gradient is zero, whatever stands in g there.
  * second:   with r, rtable the cotangents of glogits, gtable (null: zero), the derivatives with respect to alpha and g;
- *           null outputs are skipped. */
+ *           null outputs are skipped.  The one with respect to alpha is for rows of alpha that sum to one: a constant of a row, which
+ *           the backward of alpha takes out, is left out of it.
+ * halpha is what the backward then takes as g.  It is a difference, too: in 16 bits its rounding counts many times, and it may be
+ * beyond their range where the gradients are not.  The `_wide` forms write halpha, and take g, in float for the 16-bit types (aligned to
+ * 16 bytes); for the other types they are the same calls. */
 typedef struct {
   int64_t num_rows, num_edges, num_pieces, num_cut;
   const int32_t* rowptr;
@@ -325,9 +329,15 @@ LUNA_API int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, const
 LUNA_API int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g,
                                     const int32_t* buckets, void* glogits, void* gtable, int64_t heads, int64_t num_buckets,
                                     void* scratch, int64_t scratch_bytes, void* stream);
+LUNA_API int luna_graph_softmax_bwd_wide(int dtype, const luna_row_table* rows, const void* alpha, const void* g,
+                                         const int32_t* buckets, void* glogits, void* gtable, int64_t heads, int64_t num_buckets,
+                                         void* scratch, int64_t scratch_bytes, void* stream);
 LUNA_API int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
                                         const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
                                         int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream);
+LUNA_API int luna_graph_softmax_dbl_bwd_wide(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
+                                             const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
+                                             int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* --------------------------------------------------------------------------------------------------------------
  * Measurement aid, no counterpart in the reference: launches register-resident chains of fused multiply-adds

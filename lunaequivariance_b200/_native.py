@@ -148,6 +148,10 @@ _SIGNATURES = {
                                               ctypes.c_int64, _P]),
     "luna_graph_softmax_bwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
                                               ctypes.c_int64, _P]),
+    "luna_graph_softmax_bwd_wide": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 5, *[ctypes.c_int64] * 2, _P,
+                                                   ctypes.c_int64, _P]),
+    "luna_graph_softmax_dbl_bwd_wide": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 7, *[ctypes.c_int64] * 2,
+                                                       _P, ctypes.c_int64, _P]),
     "luna_graph_softmax_dbl_bwd": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RowTable), *[_P] * 7, *[ctypes.c_int64] * 2,
                                                   _P, ctypes.c_int64, _P]),
 }

@@ -119,9 +119,11 @@ extern "C" int luna_graph_softmax_fwd(int dtype, const luna_row_table* rows, con
   return status;
 }
 
-extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const int32_t* buckets,
-                                      void* glogits, void* gtable, int64_t heads, int64_t num_buckets, void* scratch,
-                                      int64_t scratch_bytes, void* stream) {
+namespace {
+
+// wide: g in float for the 16-bit types
+int backward(int dtype, const luna_row_table* rows, const void* alpha, const void* g, bool wide_g, const int32_t* buckets, void* glogits,
+             void* gtable, int64_t heads, int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
   const Call call{dtype, rows, heads, num_buckets, buckets};
@@ -130,7 +132,7 @@ extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, con
   if (status) return status;
   const bool any = rows->num_edges > 0;
   if ((status = softmax::wide_pointer(call, alpha, "alpha", any))) return status;
-  if ((status = softmax::pointer(call, g, "g", any))) return status;
+  if ((status = wide_g ? softmax::wide_pointer(call, g, "g", any) : softmax::pointer(call, g, "g", any))) return status;
   if ((status = softmax::pointer(call, glogits, "glogits", any))) return status;
   if ((status = softmax::pointer(call, gtable, "gtable", false))) return status;
   if (gtable && ((any && !buckets) || num_buckets < 1)) return fail(LUNA_ERR_INVALID_ARGUMENT, "a table needs buckets");
@@ -147,12 +149,17 @@ extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, con
     rows::with_type(dtype, [&](auto zero) {
       using T = decltype(zero);
       softmax::Operands<T> o{};
+      const bool widened = wide_g && sizeof(T) == 2;
       o.alpha = static_cast<const rows::Acc<T>*>(alpha);
       o.g = static_cast<const T*>(g);
+      o.gwide = static_cast<const rows::Acc<T>*>(g);
       o.out = static_cast<T*>(glogits);
       o.wide = static_cast<rows::Acc<T>*>(wide);
-      const int vec = sizeof(T) == 2 ? bias::packet_of(sizeof(T), heads, {g, glogits}) : bias::packet_of(sizeof(T), heads, {alpha, g, glogits});
-      status = softmax::run<T>(softmax::kBackward, vec, R, rows->num_edges, heads, num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
+      const int vec = widened          ? bias::packet_of(sizeof(T), heads, {glogits})
+                      : sizeof(T) == 2 ? bias::packet_of(sizeof(T), heads, {g, glogits})
+                                       : bias::packet_of(sizeof(T), heads, {alpha, g, glogits});
+      status = softmax::run<T>(widened ? softmax::kBackwardWide : softmax::kBackward, vec, R, rows->num_edges, heads, num_buckets, o, scratch,
+                               static_cast<cudaStream_t>(stream));
     });
   if (status || !gtable) return status;
   rows::with_type(dtype, [&](auto zero) {
@@ -167,9 +174,10 @@ extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, con
   return status;
 }
 
-extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
-                                          const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
-                                          int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
+// wide: halpha in float for the 16-bit types
+int second_order(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r, const void* rtable,
+                 const int32_t* buckets, void* halpha, bool wide_halpha, void* hg, int64_t heads, int64_t num_buckets, void* scratch,
+                 int64_t scratch_bytes, void* stream) {
   using namespace luna;
   clear_error();
   const Call call{dtype, rows, heads, num_buckets, buckets};
@@ -181,7 +189,7 @@ extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows,
   if ((status = softmax::pointer(call, g, "g", any))) return status;
   if ((status = softmax::pointer(call, r, "r", false))) return status;
   if ((status = softmax::pointer(call, rtable, "rtable", false))) return status;
-  if ((status = softmax::pointer(call, halpha, "halpha", false))) return status;
+  if ((status = wide_halpha ? softmax::wide_pointer(call, halpha, "halpha", false) : softmax::pointer(call, halpha, "halpha", false))) return status;
   if ((status = softmax::pointer(call, hg, "hg", false))) return status;
   if (rtable && any && (!buckets || num_buckets < 1)) return fail(LUNA_ERR_INVALID_ARGUMENT, "a table needs buckets");
   if ((status = softmax::scratch_fits(softmax::pieces_bytes(call), scratch, scratch_bytes))) return status;
@@ -195,10 +203,36 @@ extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows,
     o.rtable = static_cast<const T*>(rtable);
     o.buckets = buckets;
     o.out = static_cast<T*>(hg);
-    o.out2 = static_cast<T*>(halpha);
+    if (wide_halpha && sizeof(T) == 2)
+      o.wide = static_cast<rows::Acc<T>*>(halpha);  // aligned to 16 bytes: to whole packets of T, whatever they are
+    else
+      o.out2 = static_cast<T*>(halpha);
     const int vec = sizeof(T) == 2 ? bias::packet_of(sizeof(T), heads, {g, r, rtable, halpha, hg})
                                    : bias::packet_of(sizeof(T), heads, {alpha, g, r, rtable, halpha, hg});
     status = softmax::run<T>(softmax::kSecond, vec, R, rows->num_edges, heads, num_buckets, o, scratch, static_cast<cudaStream_t>(stream));
   });
   return status;
+}
+
+}  // namespace
+
+extern "C" int luna_graph_softmax_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const int32_t* buckets,
+                                      void* glogits, void* gtable, int64_t heads, int64_t num_buckets, void* scratch,
+                                      int64_t scratch_bytes, void* stream) {
+  return backward(dtype, rows, alpha, g, false, buckets, glogits, gtable, heads, num_buckets, scratch, scratch_bytes, stream);
+}
+extern "C" int luna_graph_softmax_bwd_wide(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const int32_t* buckets,
+                                           void* glogits, void* gtable, int64_t heads, int64_t num_buckets, void* scratch,
+                                           int64_t scratch_bytes, void* stream) {
+  return backward(dtype, rows, alpha, g, true, buckets, glogits, gtable, heads, num_buckets, scratch, scratch_bytes, stream);
+}
+extern "C" int luna_graph_softmax_dbl_bwd(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
+                                          const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
+                                          int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
+  return second_order(dtype, rows, alpha, g, r, rtable, buckets, halpha, false, hg, heads, num_buckets, scratch, scratch_bytes, stream);
+}
+extern "C" int luna_graph_softmax_dbl_bwd_wide(int dtype, const luna_row_table* rows, const void* alpha, const void* g, const void* r,
+                                               const void* rtable, const int32_t* buckets, void* halpha, void* hg, int64_t heads,
+                                               int64_t num_buckets, void* scratch, int64_t scratch_bytes, void* stream) {
+  return second_order(dtype, rows, alpha, g, r, rtable, buckets, halpha, true, hg, heads, num_buckets, scratch, scratch_bytes, stream);
 }

@@ -3,8 +3,11 @@
 // Edges are sorted by destination, so a row is a contiguous piece of the [edges, heads] arrays.  With z = logit + table[bucket]
 // (masked edges: -inf), m = max z and l = sum exp(z - m) over the row: alpha = exp(z - m) / l, zeros where nothing is left.
 //   backward   with D = sum alpha g:   dz = alpha (g - D)
-//   second     the cotangent r of dz, R = sum alpha r:   d/dg = alpha (r - R),   d/dalpha = r (g - D) - g R
-// Where alpha is zero nothing flows, whatever stands in g or r there.
+//   second     the cotangent r of dz, R = sum alpha r:   d/dg = alpha (r - R),   d/dalpha = (g - D) (r - R)
+// Where alpha is zero nothing flows, whatever stands in g or r there.  d/dalpha is meant for an alpha whose rows sum to one: it is
+// r (g - D) - g R and the row's constant D R, which the backward takes out with D.  Made of the distances from the means: the
+// products of g and r themselves are as large as their squares, and what is left of them behind the constant may be nothing but
+// rounding: of g and r with a spread of one about 1000, FP32, dz was off by 17 % of its largest (0.01 % like this).
 //
 // Bound by HBM: a row's values are read once and held in registers between its sums and its outputs, as far as they fit (K packets
 // of a thread); the rest of a longer row passes twice, the second time from cache.  All loads of a batch are under way before
@@ -36,7 +39,8 @@ struct Shape {
   int num_buckets;
 };
 
-enum Order { kForward, kBackward, kSecond };
+enum Order { kForward, kBackward, kSecond, kBackwardWide };  // the last: kBackward with `gwide` in place of `g`, for the 16-bit types
+constexpr bool is_backward(int order) { return order == kBackward || order == kBackwardWide; }
 enum Phase { kWhole, kMixed, kApply };  // no pieces; whole rows and the pieces' sums; the pieces' outputs
 
 template <typename T>
@@ -44,10 +48,11 @@ struct Operands {
   const T *logits, *table;
   const Acc<T>* alpha;  // as the sums are held: rounded to 16 bits, the sums by bucket of alpha (g - D) are off by more than their own rounding
   const T *g, *r, *rtable;
+  const Acc<T>* gwide;
   const int32_t* buckets;
   const uint8_t* mask;
   T *out, *out2;
-  Acc<T>* wide;  // 16-bit types: the output once more, as it was before it was rounded
+  Acc<T>* wide;  // 16-bit types: the output (of the second order, d/dalpha) as it was before it was rounded
 };
 
 template <typename A>
@@ -130,7 +135,7 @@ __device__ __forceinline__ A taken(A largest) {
 
 // LANES: as S.lanes, where an edge's heads fill their `across` packets, so that a row is one stretch of packets; 0: neither is known.
 template <typename T, int VEC, int K, int ORDER, int PHASE, int LANES>
-__global__ void __launch_bounds__(kThreads, ORDER == kBackward ? 4 : ORDER == kForward && sizeof(T) <= 4 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, is_backward(ORDER) ? 4 : ORDER == kForward && sizeof(T) <= 4 ? 3 : 2)
 rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __restrict__ stats) {
   using A = Acc<T>;
   using In = rows::Pack<T, VEC>;
@@ -180,7 +185,10 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
       bring(o.logits, u, lowest<A>());
     } else {
       bring(o.alpha, u, A(0));
-      bring(o.g, g, A(0));
+      if constexpr (ORDER == kBackwardWide)
+        bring(o.gwide, g, A(0));
+      else
+        bring(o.g, g, A(0));
       if constexpr (ORDER == kSecond) {
         if (o.r) {
           bring(o.r, r, A(0));
@@ -228,18 +236,21 @@ rows_kernel(const Rows R, const Shape S, const Operands<T> o, Pair<Acc<T>>* __re
         const A alpha = u[k][c];
         if constexpr (ORDER == kForward) {
           v[c] = alpha * b[c];
-        } else if constexpr (ORDER == kBackward) {
+        } else if constexpr (is_backward(ORDER)) {
           v[c] = alpha != A(0) ? alpha * (g[k][c] - a[c]) : A(0);
         } else {
           v[c] = alpha != A(0) ? alpha * (r[k][c] - b[c]) : A(0);
-          w[c] = alpha != A(0) ? r[k][c] * (g[k][c] - a[c]) - g[k][c] * b[c] : A(0);
+          w[c] = alpha != A(0) ? (g[k][c] - a[c]) * (r[k][c] - b[c]) : A(0);
         }
       }
       if (ORDER != kSecond || o.out) rows::store<T, VEC>(out + k * stride, v);
       if constexpr (sizeof(T) == 2 && ORDER != kSecond)
         if (o.wide) rows::store<A, VEC>(o.wide + at + k * stride, v);
-      if constexpr (ORDER == kSecond)
+      if constexpr (ORDER == kSecond) {
         if (o.out2) rows::store<T, VEC>(out2 + k * stride, w);
+        if constexpr (sizeof(T) == 2)
+          if (o.wide) rows::store<A, VEC>(o.wide + at + k * stride, w);
+      }
     }
     if constexpr (ORDER == kForward) {
       // Zero times a sum that is no number is none either: what is masked beside one is put right, a walk that no other row takes.
@@ -437,7 +448,7 @@ template <typename T, int VEC, int ORDER>
 int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch, cudaStream_t stream) {
   // Sixteen numbers of a thread in registers; single ones, with their exponentials and addresses, spill (forward, 2.6 M edges
   // with one head: 23 us, with eight 14; the backward has room: 8.3 and 9.8).
-  constexpr int K = sizeof(T) > 4 ? 8 / VEC : VEC == 1 && ORDER != kBackward ? 8 : 16 / VEC;
+  constexpr int K = sizeof(T) > 4 ? 8 / VEC : VEC == 1 && !is_backward(ORDER) ? 8 : 16 / VEC;
   Shape S{};
   S.heads = static_cast<int>(heads);
   S.num_buckets = static_cast<int>(num_buckets);
@@ -478,6 +489,9 @@ int run(Order order, int vec, const Rows& R, int64_t edges, int64_t heads, int64
         cudaStream_t stream) {
   if (order == kForward) return with_packets<T, kForward>(vec, R, edges, heads, num_buckets, o, scratch, stream);
   if (order == kBackward) return with_packets<T, kBackward>(vec, R, edges, heads, num_buckets, o, scratch, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (order == kBackwardWide) return with_packets<T, kBackwardWide>(vec, R, edges, heads, num_buckets, o, scratch, stream);
+  }
   return with_packets<T, kSecond>(vec, R, edges, heads, num_buckets, o, scratch, stream);
 }
 

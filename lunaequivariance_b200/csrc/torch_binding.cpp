@@ -56,8 +56,8 @@ struct Api {
   decltype(&luna_relative_bias_bwd) bias_bwd = nullptr;
   decltype(&luna_graph_softmax_scratch_bytes) softmax_scratch_bytes = nullptr;
   decltype(&luna_graph_softmax_fwd) softmax_fwd = nullptr;
-  decltype(&luna_graph_softmax_bwd) softmax_bwd = nullptr;
-  decltype(&luna_graph_softmax_dbl_bwd) softmax_dbl_bwd = nullptr;
+  decltype(&luna_graph_softmax_bwd) softmax_bwd = nullptr, softmax_bwd_wide = nullptr;
+  decltype(&luna_graph_softmax_dbl_bwd_wide) softmax_dbl_bwd_wide = nullptr;
 } api;
 
 template <typename F>
@@ -93,7 +93,8 @@ void load(const std::string& path) {
   resolve(library, "luna_graph_softmax_scratch_bytes", api.softmax_scratch_bytes);
   resolve(library, "luna_graph_softmax_fwd", api.softmax_fwd);
   resolve(library, "luna_graph_softmax_bwd", api.softmax_bwd);
-  resolve(library, "luna_graph_softmax_dbl_bwd", api.softmax_dbl_bwd);
+  resolve(library, "luna_graph_softmax_bwd_wide", api.softmax_bwd_wide);
+  resolve(library, "luna_graph_softmax_dbl_bwd_wide", api.softmax_dbl_bwd_wide);
 }
 
 // A failed status as the exception Python raises for it.
@@ -1083,7 +1084,8 @@ void check_table(const Tensor& x, const Tensor& table, const Tensor& buckets) {
   check_beside(x, buckets, "buckets", {x.size(0)}, at::kInt);
 }
 
-bool narrow(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+bool narrow(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+bool narrow(const Tensor& t) { return narrow(t.scalar_type()); }
 
 // alpha, and what the backward makes gradients of: alpha itself, or for the 16-bit types alpha before it was rounded.
 std::array<Tensor, 2> softmax_forward(const Rows& rows, const Tensor& logits, const Tensor& table, const Tensor& buckets, const Tensor& mask,
@@ -1104,60 +1106,69 @@ std::array<Tensor, 2> softmax_forward(const Rows& rows, const Tensor& logits, co
   return {alpha, wide};
 }
 
-// What the launches read alpha from: `wide` where there is one.  Other alphas of 16 bits are what a caller of the operators has made.
-Tensor exact_alpha(const Tensor& alpha, const Tensor& wide) {
-  if (!narrow(alpha)) return alpha.contiguous();
-  if (!wide.defined() || !wide.numel()) return alpha.to(at::kFloat).contiguous();
-  check_beside(alpha, wide, "wide", alpha.sizes(), at::kFloat);
-  return wide.contiguous();
+// In what follows `alpha` is as the launches read it, in float for the 16-bit types, and `type` is the operator's type.  Its cotangent is
+// of either: of `type` from a loss, and as wide as alpha from the second order, whose differences 16 bits may not hold.
+void check_alpha(const Rows& rows, const Tensor& alpha, at::ScalarType type, const Tensor& g) {
+  check_softmax(rows, alpha, "alpha");
+  refuse_tangents({&g});
+  TORCH_CHECK_TYPE(alpha.scalar_type() == (narrow(type) ? at::kFloat : type), "alpha must be ", narrow(type) ? at::kFloat : type, ", got ",
+                   alpha.scalar_type());
+  check_beside(alpha, g, "grad_out", alpha.sizes(), g.scalar_type() == alpha.scalar_type() ? alpha.scalar_type() : type);
 }
+int code_of(at::ScalarType type) { return type == at::kDouble ? LUNA_F64 : type == at::kFloat ? LUNA_F32 : type == at::kHalf ? LUNA_F16 : LUNA_BF16; }
 
 // The gradients of the logits and of the table, as far as `mask` names them.
-std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, const Tensor& wide, const Tensor& g, const Tensor& buckets,
+std::array<Tensor, 2> softmax_backward(const Rows& rows, const Tensor& alpha, at::ScalarType type, const Tensor& g, const Tensor& buckets,
                                        int64_t num_buckets, int mask) {
   std::array<Tensor, 2> out;
   if (!mask) return out;
-  const int dtype = check_softmax(rows, alpha, "alpha");
-  refuse_tangents({&g});
-  check_beside(alpha, g, "grad_out", alpha.sizes());
+  check_alpha(rows, alpha, type, g);
   check_table(alpha, Tensor(), buckets);
   const c10::cuda::CUDAGuard guard(alpha.device());
-  const Tensor a = exact_alpha(alpha, wide), e = g.contiguous(), b = contiguous(buckets);
-  out[0] = at::empty(e.sizes(), e.options());  // the table's gradient is made of it
-  if (mask & 2) out[1] = at::empty({num_buckets, heads_of(e)}, e.options());
+  const Tensor a = prepared(alpha), e = prepared(g), b = contiguous(buckets);
+  const auto options = a.options().dtype(type);
+  out[0] = at::empty(e.sizes(), options);  // the table's gradient is made of it
+  if (mask & 2) out[1] = at::empty({num_buckets, heads_of(e)}, options);
+  const int dtype = code_of(type);
   const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(e), mask & 2 ? num_buckets : 0), e);
-  check(api.softmax_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), static_cast<const int32_t*>(pointer(b)), out[0].data_ptr(),
-                        pointer(out[1]), heads_of(e), num_buckets, pointer(scratch), bytes_of(scratch), stream_of(e)));
+  const auto entry = e.scalar_type() == type ? api.softmax_bwd : api.softmax_bwd_wide;
+  check(entry(dtype, &rows.native, a.data_ptr(), e.data_ptr(), static_cast<const int32_t*>(pointer(b)), out[0].data_ptr(), pointer(out[1]),
+              heads_of(e), num_buckets, pointer(scratch), bytes_of(scratch), stream_of(e)));
   if (!(mask & 1)) out[0] = Tensor();
   return out;
 }
 
-// The derivatives with respect to alpha and g named in `mask`.
-std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, const Tensor& wide, const Tensor& g, const Tensor& buckets,
+// The derivatives with respect to alpha, as wide as it is, and g named in `mask`.
+std::array<Tensor, 2> softmax_double(const Rows& rows, const Tensor& alpha, at::ScalarType type, const Tensor& g, const Tensor& buckets,
                                      const Tensor& r, const Tensor& rtable, int mask) {
   std::array<Tensor, 2> out;
   if (!mask) return out;
-  const int dtype = check_softmax(rows, alpha, "alpha");
-  refuse_tangents({&g, &r, &rtable});
-  check_beside(alpha, g, "grad_out", alpha.sizes());
-  check_beside(alpha, r, "r", alpha.sizes());
-  check_table(alpha, rtable, buckets);
+  check_alpha(rows, alpha, type, g);
+  refuse_tangents({&r, &rtable});
+  check_beside(alpha, r, "r", alpha.sizes(), type);
+  check_table(alpha, Tensor(), buckets);
+  if (rtable.defined()) check_beside(alpha, rtable, "table", {rtable.size(0), heads_of(alpha)}, type);
   const c10::cuda::CUDAGuard guard(alpha.device());
-  const Tensor a = exact_alpha(alpha, wide), e = g.contiguous(), b = contiguous(buckets), t = contiguous(r), tt = contiguous(rtable);
-  for (int s = 0; s < 2; ++s)
-    if (mask >> s & 1) out[s] = at::empty(e.sizes(), e.options());
+  auto widened = [&](const Tensor& t) { return t.defined() ? t.to(alpha.scalar_type()) : t; };
+  if (g.scalar_type() != type)  // the backward of a second order's cotangent: in the type of the sums altogether
+    return softmax_double(rows, alpha, alpha.scalar_type(), g, buckets, widened(r), widened(rtable), mask);
+  const Tensor a = prepared(alpha), e = g.contiguous(), b = contiguous(buckets), t = contiguous(r), tt = contiguous(rtable);
+  if (mask & 1) out[0] = at::empty(a.sizes(), a.options());
+  if (mask & 2) out[1] = at::empty(e.sizes(), e.options());
+  const int dtype = code_of(type);
   const Tensor scratch = scratch_of(api.softmax_scratch_bytes(dtype, &rows.native, heads_of(e), 0), e);
-  check(api.softmax_dbl_bwd(dtype, &rows.native, a.data_ptr(), e.data_ptr(), pointer(t), pointer(tt), static_cast<const int32_t*>(pointer(b)),
-                            pointer(out[0]), pointer(out[1]), heads_of(e), tt.defined() ? tt.size(0) : 0, pointer(scratch), bytes_of(scratch),
-                            stream_of(e)));
+  check(api.softmax_dbl_bwd_wide(dtype, &rows.native, a.data_ptr(), e.data_ptr(), pointer(t), pointer(tt),
+                                 static_cast<const int32_t*>(pointer(b)), pointer(out[0]), pointer(out[1]), heads_of(e),
+                                 tt.defined() ? tt.size(0) : 0, pointer(scratch), bytes_of(scratch), stream_of(e)));
   return out;
 }
 
 struct SoftmaxDouble : Function<SoftmaxDouble> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& wide, const Maybe& buckets,
-                               const Maybe& r, const Maybe& rtable, int64_t mask, const RowsPtr& rows) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, const Maybe& r,
+                               const Maybe& rtable, int64_t type, int64_t mask, const RowsPtr& rows) {
     ctx->set_materialize_grads(false);
-    return only(softmax_double(*rows, alpha, of(wide), g, of(buckets), of(r), of(rtable), static_cast<int>(mask)), static_cast<int>(mask));
+    return only(softmax_double(*rows, alpha, static_cast<at::ScalarType>(type), g, of(buckets), of(r), of(rtable), static_cast<int>(mask)),
+                static_cast<int>(mask));
   }
   static variable_list backward(AutogradContext*, const variable_list& grads) {
     for (const Tensor& t : grads)
@@ -1167,13 +1178,15 @@ struct SoftmaxDouble : Function<SoftmaxDouble> {
 };
 
 struct SoftmaxBackward : Function<SoftmaxBackward> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& wide, const Maybe& buckets,
-                               int64_t num_buckets, int64_t mask, const RowsPtr& rows) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& alpha, const Tensor& g, const Maybe& buckets, int64_t num_buckets,
+                               int64_t type, int64_t mask, const RowsPtr& rows) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({alpha, g, of(wide), of(buckets)});
+    ctx->save_for_backward({alpha, g, of(buckets)});
+    ctx->saved_data["type"] = type;
     ctx->saved_data["mask"] = mask;
     keep(ctx, "rows", rows);
-    return only(softmax_backward(*rows, alpha, of(wide), g, of(buckets), num_buckets, static_cast<int>(mask)), static_cast<int>(mask));
+    return only(softmax_backward(*rows, alpha, static_cast<at::ScalarType>(type), g, of(buckets), num_buckets, static_cast<int>(mask)),
+                static_cast<int>(mask));
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(7);
@@ -1183,46 +1196,60 @@ struct SoftmaxBackward : Function<SoftmaxBackward> {
     const int mask = wanted(ctx, {&saved[0], &saved[1]});
     if (!mask) return out;
     const auto rows = kept<Rows>(ctx, "rows");
+    const int64_t type = ctx->saved_data["type"].toInt();
     const auto h = at::GradMode::is_enabled()
-                       ? spread<2>(SoftmaxDouble::apply(saved[0], saved[1], maybe(saved[2]), maybe(saved[3]), maybe(r[0]), maybe(r[1]),
+                       ? spread<2>(SoftmaxDouble::apply(saved[0], saved[1], maybe(saved[2]), maybe(r[0]), maybe(r[1]), type,
                                                         static_cast<int64_t>(mask), rows), mask)
-                       : softmax_double(*rows, saved[0], saved[2], saved[1], saved[3], r[0], r[1], mask);
+                       : softmax_double(*rows, saved[0], static_cast<at::ScalarType>(type), saved[1], saved[2], r[0], r[1], mask);
     for (int s = 0; s < 2; ++s) out[s] = h[s];
     return out;
   }
 };
 
+// For the 16-bit types alpha as it was before it was rounded is an output of its own, which no caller sees: the second order's cotangent
+// of alpha comes back through it, as wide as it was made.
 struct SoftmaxForward : Function<SoftmaxForward> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask,
-                        const RowsPtr& rows) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask,
+                               const RowsPtr& rows) {
     const auto found = softmax_forward(*rows, logits, of(table), of(buckets), of(mask), true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({found[0], found[1], of(buckets)});  // alpha says all about the logits, the table and the mask
+    const bool rounded = found[1].defined();
+    ctx->save_for_backward({found[rounded ? 1 : 0], of(buckets)});  // alpha says all about the logits, the table and the mask
     ctx->saved_data["buckets"] = table ? table->size(0) : 0;
+    ctx->saved_data["type"] = static_cast<int64_t>(logits.scalar_type());
     keep(ctx, "rows", rows);
-    return found[0];
+    return rounded ? variable_list{found[0], found[1]} : variable_list{found[0]};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(5);
-    if (!grads[0].defined()) return out;
+    Tensor g = grads[0];
+    if (grads.size() > 1 && grads[1].defined()) g = g.defined() ? grads[1] + g : grads[1];
+    if (!g.defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    const int64_t num_buckets = ctx->saved_data["buckets"].toInt();
+    const int64_t num_buckets = ctx->saved_data["buckets"].toInt(), type = ctx->saved_data["type"].toInt();
     int mask = ctx->needs_input_grad(0) ? 1 : 0;
     if (num_buckets && ctx->needs_input_grad(1)) mask |= 2;
     if (!mask) return out;
     const auto rows = kept<Rows>(ctx, "rows");
     const auto d = at::GradMode::is_enabled()
-                       ? spread<2>(SoftmaxBackward::apply(saved[0], grads[0], maybe(saved[1]), maybe(saved[2]), num_buckets,
-                                                          static_cast<int64_t>(mask), rows), mask)
-                       : softmax_backward(*rows, saved[0], saved[1], grads[0], saved[2], num_buckets, mask);
+                       ? spread<2>(SoftmaxBackward::apply(saved[0], g, maybe(saved[1]), num_buckets, type, static_cast<int64_t>(mask), rows), mask)
+                       : softmax_backward(*rows, saved[0], static_cast<at::ScalarType>(type), g, saved[1], num_buckets, mask);
     for (int s = 0; s < 2; ++s) out[s] = d[s];
     return out;
   }
 };
 
+// What the launches read alpha from, for a caller of the operators: `wide` where there is one.
+Tensor exact_alpha(const Tensor& alpha, const Tensor& wide) {
+  if (!narrow(alpha)) return alpha;
+  if (!wide.defined() || !wide.numel()) return alpha.to(at::kFloat);
+  check_beside(alpha, wide, "wide", alpha.sizes(), at::kFloat);
+  return wide;
+}
+
 Tensor graph_softmax(const RowsPtr& rows, const Tensor& logits, const Maybe& table, const Maybe& buckets, const Maybe& mask) {
   pybind11::gil_scoped_release release;
-  return tracked({&logits, &of(table)}) ? SoftmaxForward::apply(logits, table, buckets, mask, rows)
+  return tracked({&logits, &of(table)}) ? SoftmaxForward::apply(logits, table, buckets, mask, rows)[0]
                                         : softmax_forward(*rows, logits, of(table), of(buckets), of(mask), false)[0];
 }
 
@@ -1269,10 +1296,10 @@ PYBIND11_MODULE(luna_torch, m) {
   }));
   m.def("graph_softmax_backward", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Maybe& wide, const Tensor& g,
                                                                  const Maybe& buckets, int64_t num_buckets, int mask) {
-    return listed(softmax_backward(*rows, alpha, of(wide), g, of(buckets), num_buckets, mask));
+    return listed(softmax_backward(*rows, exact_alpha(alpha, of(wide)), alpha.scalar_type(), g, of(buckets), num_buckets, mask));
   }));
   m.def("graph_softmax_double", torch::wrap_pybind_function([](const RowsPtr& rows, const Tensor& alpha, const Maybe& wide, const Tensor& g,
                                                                const Maybe& buckets, const Maybe& r, const Maybe& rtable, int mask) {
-    return listed(softmax_double(*rows, alpha, of(wide), g, of(buckets), of(r), of(rtable), mask));
+    return listed(softmax_double(*rows, exact_alpha(alpha, of(wide)), alpha.scalar_type(), g, of(buckets), of(r), of(rtable), mask));
   }));
 }

@@ -26,11 +26,17 @@ def _rows(rowptr, edges):
     return _native.binding().Rows(rowptr, edges, None, None, None, None)
 
 
+def _narrow(t):
+    return t.dtype in (torch.bfloat16, torch.float16)
+
+
 @torch.library.custom_op("lunaeq::graph_softmax_forward", mutates_args=(),
                          schema="(Tensor logits, Tensor? table, Tensor? buckets, Tensor? mask, Tensor rowptr, SymInt edges)"
                                 " -> (Tensor, Tensor)")
 def graph_softmax_forward_op(logits, table, buckets, mask, rowptr, edges):
-    """The result, and for 16-bit types the result before it was rounded (else nothing)."""
+    """The result, and for 16-bit types the result before it was rounded (else nothing).
+
+    The second order's cotangent of a 16-bit result comes back through the latter: its rounding would count many times."""
     alpha, wide = _native.binding().graph_softmax_forward(_rows(rowptr, edges), logits, table, buckets, mask)
     return alpha, logits.new_empty(0, dtype=torch.float32) if wide is None else wide
 
@@ -38,8 +44,7 @@ def graph_softmax_forward_op(logits, table, buckets, mask, rowptr, edges):
 @graph_softmax_forward_op.register_fake
 def _(logits, table, buckets, mask, rowptr, edges):
     alpha = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    narrow = logits.dtype in (torch.bfloat16, torch.float16)
-    return alpha, alpha.new_empty(alpha.shape if narrow else (0,), dtype=torch.float32)
+    return alpha, alpha.new_empty(alpha.shape if _narrow(logits) else (0,), dtype=torch.float32)
 
 
 @torch.library.custom_op("lunaeq::graph_softmax_backward", mutates_args=(),
@@ -67,18 +72,22 @@ def graph_softmax_double_backward_op(alpha, wide, g, buckets, r, rtable, rowptr,
 
 @graph_softmax_double_backward_op.register_fake
 def _(alpha, wide, g, buckets, r, rtable, rowptr, needs):
-    return tuple(torch.empty_like(alpha, memory_format=torch.contiguous_format) if need else None for need in needs)
+    return (torch.empty_like(alpha, dtype=torch.float32 if _narrow(alpha) else None, memory_format=torch.contiguous_format) if needs[0] else None,
+            torch.empty_like(g, memory_format=torch.contiguous_format) if needs[1] else None)
 
 
 def _forward_setup(ctx, inputs, output):
     _, table, buckets, _, rowptr, _ = inputs
     ctx.num_buckets = 0 if table is None else table.shape[0]
     ctx.save_for_backward(*output, buckets, rowptr)
-    ctx.mark_non_differentiable(output[1])
+    if not _narrow(output[0]):
+        ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)
 
 
-def _forward_backward(ctx, g, _):
+def _forward_backward(ctx, g, wide_g):
+    if wide_g is not None:
+        g = wide_g if g is None else wide_g + g
     if g is None:
         return (None,) * 6
     alpha, wide, buckets, rowptr = ctx.saved_tensors
@@ -96,9 +105,12 @@ def _backward_backward(ctx, r, rtable):
     if r is None and rtable is None:
         return (None,) * 7
     alpha, wide, g, buckets, rowptr = ctx.saved_tensors
-    needs = [ctx.needs_input_grad[0], ctx.needs_input_grad[2]]
+    widened = _narrow(alpha) and wide.numel() > 0  # what the launches read in the place of alpha
+    needs = [ctx.needs_input_grad[1 if widened else 0], ctx.needs_input_grad[2]]
     halpha, hg = graph_softmax_double_backward_op(alpha, wide, g, buckets, r, rtable, rowptr, needs)
-    return halpha, None, hg, None, None, None, None
+    if widened:
+        return None, halpha, hg, None, None, None, None
+    return None if halpha is None else halpha.to(alpha.dtype), None, hg, None, None, None, None
 
 
 graph_softmax_forward_op.register_autograd(_forward_backward, setup_context=_forward_setup)

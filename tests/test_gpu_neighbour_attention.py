@@ -68,3 +68,84 @@ def test_what_is_masked_stays_zero_beside_what_is_no_number(rows, heads, dtype):
         fine = ~bad[dst] & mask[:, None]
         assert torch.equal(a[fine], b[fine])
     assert not got[2][0].any() and not got[2][0].isnan().any()
+
+
+def softmax_orders(softmax, z, t, g, r, rt):
+    z, t, g = (v.clone().requires_grad_(True) for v in (z, t, g))
+    alpha = softmax(z, t)
+    gz, gt = torch.autograd.grad(alpha, (z, t), g, create_graph=True)
+    hz, ht, hg = torch.autograd.grad((gz, gt), (z, t, g), (r, rt))
+    return {k: v.detach() for k, v in dict(alpha=alpha, gz=gz, gt=gt, hz=hz, ht=ht, hg=hg).items()}
+
+
+@pytest.mark.parametrize("dtype,shift,spread", [(BF16, 0, 1), (BF16, 3, 1), (BF16, 10, 1), (BF16, 0, 300), (F16, 0, 100), (F16, 100, 30), (F16, 10, 1),
+                                                (F32, 0, 1), (F32, 1e5, 1), (F64, 1e6, 1)])
+@pytest.mark.parametrize("rows,heads", [("short", 3), ("warps", 8), ("warps", 1), ("ctas", 4), ("cut", 2)])
+def test_second_order_of_the_softmax_far_from_zero(rows, heads, dtype, shift, spread):
+    """Cotangents that are far from zero, or large: the second order is made of their distances from the row's means.
+
+    With D, R the means of g and r by alpha, sg, sr the largest distances from them and G, R the largest cotangents:
+    hz = alpha ((g - D)(r - R) - their mean).  alpha, the means and their sums are off by `relative` of what goes into them: the exponent's
+    size, 64 additions one after the other and thirty operations.  So a distance is off by relative G, and a product by relative (G sr + sg R +
+    sg sr + relative G R); it is there twice, itself and in the mean, and alpha's own error weighs the same once more: eight of them are above all.
+    """
+    generator = torch.Generator().manual_seed(heads)
+    degrees = ROWS[rows]
+    graph, dst = graph_of(degrees, generator)
+    nodes, edges, count = len(degrees), dst.numel(), 5
+    rand = lambda *shape: torch.randn(*shape, generator=generator, dtype=F64)  # noqa: E731
+    p = [t.to(dtype) for t in (2 * rand(edges, heads), rand(count, heads), shift + spread * rand(edges, heads), shift + spread * rand(edges, heads),
+                               0 * rand(count, heads))]
+    mask = torch.rand(edges, generator=generator) < 0.8
+    buckets = torch.randint(-1, count, (edges,), generator=generator, dtype=torch.int32)
+    # a constant in all of g or of r changes nothing, so the definition is asked without it
+    want = softmax_orders(lambda z, t: oracle.graph_softmax(z, dst, nodes, mask, t, buckets),
+                          *(t.double() - c for t, c in zip(p, (0, 0, shift, shift, 0))))
+    got = softmax_orders(lambda z, t: luna.graph_softmax(z, graph, mask=mask.to(DEVICE), table=t, buckets=buckets.to(DEVICE)),
+                         *(t.to(DEVICE) for t in p))
+    z, t, g, r, _ = (v.double() for v in p)
+    span = z.abs().max() + t.abs().max()
+    relative = inner(dtype) * (4 * span + 64 + 30)
+    alpha = want["alpha"]
+
+    def mean(v):
+        return torch.zeros(nodes, heads, dtype=F64).index_add_(0, dst, alpha * v)[dst]
+
+    def largest(v):
+        return torch.zeros(nodes, heads, dtype=F64).index_reduce_(0, dst, torch.where(mask[:, None], v.abs(), 0.0), "amax")[dst]
+
+    G, R, sg, sr = largest(g), largest(r), largest(g - mean(g)), largest(r - mean(r))
+    tiny = 2.0 ** -24 if dtype == F16 else 1e-30 if dtype != F64 else 1e-300
+    error = {"gz": 4 * relative * alpha * G, "hg": 4 * relative * alpha * R, "hz": 8 * relative * alpha * (G * sr + sg * R + sg * sr + relative * G * R)}
+    for k, allowed in error.items():
+        over = (got[k].cpu().double() - want[k]).abs() / (step(dtype) * want[k].abs() + allowed + tiny)
+        assert got[k].dtype == dtype and over.max().item() <= 1.0, f"{k}: {over.max().item():.3g} of what is allowed"
+    for k, source in (("gt", "gz"), ("ht", "hz")):
+        # by bucket: the parts' errors, and 200 additions of them one after the other
+        inside = buckets >= 0
+        parts = (error[source] + 200 * inner(dtype) * want[source].abs())[inside]
+        allowed = torch.zeros(count, heads, dtype=F64).index_add_(0, buckets[inside].long(), parts) + step(dtype) * want[k].abs() + tiny
+        over = (got[k].cpu().double() - want[k]).abs() / allowed
+        assert got[k].dtype == dtype and over.max().item() <= 1.0, f"{k}: {over.max().item():.3g} of what is allowed"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_both_orders_in_one_pass(dtype):
+    """A loss of alpha and of its gradient: both cotangents of alpha meet before the logits' gradient is rounded."""
+    generator = torch.Generator().manual_seed(1)
+    graph, dst = graph_of([30] * 20, generator)
+    z, g, r, q = ((torch.randn(600, 4, generator=generator, dtype=F64)).to(dtype) for _ in range(4))
+
+    def run(softmax, z, g, r, q):
+        z, g = z.clone().requires_grad_(True), g.clone().requires_grad_(True)
+        alpha = softmax(z)
+        gz, = torch.autograd.grad(alpha, z, g, create_graph=True)
+        return torch.autograd.grad((alpha, gz), z, (q, r))[0].detach()
+
+    want = run(lambda z: oracle.graph_softmax(z, dst, 20), *(t.double() for t in (z, g, r, q)))
+    got = run(lambda z: luna.graph_softmax(z, graph), *(t.to(DEVICE) for t in (z, g, r, q)))
+    alpha = oracle.graph_softmax(z.double(), dst, 20)
+    G, R, Q = (t.double().abs().max() for t in (g, r, q))
+    # one rounding of the result; the sums' type as in the test above
+    allowed = step(dtype) * want.abs() + 8 * inner(dtype) * (4 * z.double().abs().max() + 94) * alpha * (8 * G * R + Q) + 2.0 ** -24
+    assert ((got.cpu().double() - want).abs() <= allowed).all()
