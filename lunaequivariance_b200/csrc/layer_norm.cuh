@@ -4,7 +4,7 @@
 // otherwise, s = (share |x - mu|^2 + eps)^(-1/2) with share = 1/n ("component") or 1/mul ("norm"), h = (x - mu) s, and
 // y = w_u h + b_u.  With P t = t - mean(t) - share h <h, t> (the mean for scalars only; P is symmetric) and c = w g:
 //   backward   gx = s P c,   gw_u = sum over rows and components of g h,   gb_u = sum of g
-//   second     the cotangents r of gx, rw of gw and rb of gb, q = rw g, a = <r, h>, b = <c, h>, dot = <r, c> - n mean(r) mean(c):
+//   second     the cotangents r of gx, rw of gw and rb of gb, q = rw g, a = <r, h>, b = <c, h>, dot = <r - mean(r), c - mean(c)>:
 //              hg = w s P r + rw h + rb,   hw_u = sum of s (P r) g,
 //              hx = s P q - s^2 share ((dot - share a b) h + b P r + a P c)
 //
@@ -441,7 +441,7 @@ __device__ __forceinline__ void second(const Params& P, const Block& B, int inde
   auto other = [&](const T* __restrict__ p, int offset, int k, int c) {
     return p && place.in(k) ? rows::widen(p[offset + place.channel(place.column(k) + c)]) : A(0);
   };
-  const A share = static_cast<A>(B.share), length = static_cast<A>(B.length), per_mean = B.scalar ? A(1) / length : A(0);
+  const A share = static_cast<A>(B.share), per_mean = B.scalar ? A(1) / static_cast<A>(B.length) : A(0);
   for (; row - place.ahead() < P.rows; row += step) {
     A h[K][VEC], e[K][VEC], r[K][VEC];
     const Moments<A> m = next;
@@ -450,18 +450,35 @@ __device__ __forceinline__ void second(const Params& P, const Block& B, int inde
     place.take(P, 0, o.x, row, h);
     place.take(P, 1, o.g, row, e);
     place.take(P, 2, o.rx, row, r);
-    A sums[5] = {A(0), A(0), A(0), A(0), A(0)}, more[2] = {A(0), A(0)};  // rh, ch, rc, r, c; q, qh
+    // Scalars: the means come first.  Of r and c far from zero, dot is what is left of n mean(r) mean(c), so it is made of distances
+    // (64 scalars, r and c with a spread of one about 1000, FP32: hx was off by half of its largest).  One more sum over the row, us
+    // without and with it: 1.0 M rows of 64, FP64, 458 and 461; 40,000 of 1024, FP32 142 and 154, BF16 180 and 208.  Distances from
+    // the row's first numbers need no such sum, but registers: BF16 209, three blocks of 128 270 in place of 257.
+    A mean_r = A(0), mean_c = A(0);
+    if (B.scalar) {
+      A means[2] = {A(0), A(0)};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          means[0] += r[k][c];
+          means[1] += e[k][c] * w[k][c];
+        }
+      place.sum(means);
+      mean_r = means[0] * per_mean;
+      mean_c = means[1] * per_mean;
+    }
+    A sums[3] = {A(0), A(0), A(0)}, more[2] = {A(0), A(0)};  // rh, ch, rc; q, qh
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
         h[k][c] = place.in(k) ? (h[k][c] - m.mean) * m.scale : A(0);
-        const A scaled = e[k][c] * w[k][c];
+        r[k][c] -= mean_r;
+        const A scaled = place.in(k) ? e[k][c] * w[k][c] - mean_c : A(0);  // with h zero, too, no column that is not there adds to a sum
         sums[0] += r[k][c] * h[k][c];
         sums[1] += scaled * h[k][c];
         sums[2] += r[k][c] * scaled;
-        sums[3] += r[k][c];
-        sums[4] += scaled;
         if (o.rw) {
           const A q = other(o.rw, B.weight_offset, k, c) * e[k][c];
           more[0] += q;
@@ -471,15 +488,14 @@ __device__ __forceinline__ void second(const Params& P, const Block& B, int inde
     place.sum(sums);
     if (o.rw) place.sum(more);
     if (MODE == kPackets) request(row + kStages * step);
-    const A mean_r = sums[3] * per_mean, mean_c = sums[4] * per_mean, mean_q = more[0] * per_mean;
-    const A dot = sums[2] - length * mean_r * mean_c;
+    const A mean_q = more[0] * per_mean, dot = sums[2];
     const A along_r = share * sums[0], along_c = share * sums[1], along_q = share * more[1];
     const A outer = m.scale * m.scale * share, on_h = dot - share * sums[0] * sums[1];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
-        const A p = r[k][c] - mean_r - h[k][c] * along_r;
+        const A p = r[k][c] - h[k][c] * along_r;
         const A scaled = e[k][c] * w[k][c] - mean_c - h[k][c] * along_c;
         const A from_q = on_h * h[k][c] + sums[1] * p + sums[0] * scaled;
         hw[k][c] += m.scale * p * e[k][c];  // nothing where there is no column: e is zero

@@ -149,3 +149,55 @@ def test_both_orders_in_one_pass(dtype):
     # one rounding of the result; the sums' type as in the test above
     allowed = step(dtype) * want.abs() + 8 * inner(dtype) * (4 * z.double().abs().max() + 94) * alpha * (8 * G * R + Q) + 2.0 ** -24
     assert ((got.cpu().double() - want).abs() <= allowed).all()
+
+
+@pytest.mark.parametrize("dtype,shift", [(F32, 0.0), (F32, 1e4), (F64, 1e6), (BF16, 100.0), (F16, 100.0)])
+@pytest.mark.parametrize("irreps,rows", [(3, 40), (64, 301), (50, 130), (1001, 37), (5000, 5), ("64x0e+16x1o", 100), ("32x0e+5x0o+17x0e", 33)])
+def test_second_order_of_the_layer_norm_far_from_zero(irreps, rows, dtype, shift):
+    """Cotangents with a common offset, which a block of scalars takes out: what is left depends on their distances from the mean.
+
+    With r', c' the distances of r and c = g from their means (ones as weights), R and C the largest of r and c themselves, and H the
+    largest normalised value: r' is off by a few roundings of R, so a product of r' and c' by those of R C' + C R' + R' C'.  hx is s^2
+    times such a product by h and two by a projection, |P t| <= max|t| (2 + H q) with q the root of the components; hg is s P r with
+    those of R.  A hundred roundings, as the row's sums are twenty additions and ten levels of a tree, and each output has three of them.
+    """
+    config = luna.LayerNormConfig(irreps)
+    generator = torch.Generator().manual_seed(rows)
+    rand = lambda *shape: torch.randn(*shape, generator=generator, dtype=F64)  # noqa: E731
+    x, g, r = (t.to(dtype) for t in (1.5 * rand(rows, config.dim) + 0.3, rand(rows, config.dim) + shift, rand(rows, config.dim) + shift))
+
+    def run(norm, x, g, r):
+        w = torch.ones(config.weight_numel, dtype=x.dtype, device=x.device, requires_grad=True)
+        x, g = x.clone().requires_grad_(True), g.clone().requires_grad_(True)
+        gx, = torch.autograd.grad(norm(x, w), x, g, create_graph=True)
+        return [t.detach() for t in (gx, *torch.autograd.grad(gx, (x, w, g), r))]
+
+    # a constant in a scalar block's g or r changes nothing but the weights' sums, which g is a factor of: the definition is asked without it
+    constant = torch.cat([torch.full((mul * ir.dim,), shift if ir.is_scalar() else 0.0, dtype=F64) for mul, ir in config.irreps])
+    plain = lambda x, w: oracle.layer_norm(x, config.irreps, w)  # noqa: E731
+    want = run(plain, x.double(), g.double() - constant, r.double() - constant)
+    want[2] = run(plain, x.double(), g.double(), r.double() - constant)[2]
+    got = run(lambda x, w: luna.layer_norm(x, config.irreps, w), *(t.to(DEVICE) for t in (x, g, r)))
+    at = channel = 0
+    top = lambda t: t.abs().amax(1, keepdim=True)  # noqa: E731
+    for mul, ir in config.irreps:
+        block = slice(at, at + mul * ir.dim)
+        v, e, t = (a.double()[:, block] for a in (x, g, r))
+        centred = (lambda a: a - a.mean(1, keepdim=True)) if ir.is_scalar() else (lambda a: a)
+        s = (centred(v).square().mean(1, keepdim=True) + config.eps).rsqrt()
+        H, R, C, near_r, near_c = top(centred(v) * s), top(t), top(e), top(centred(t)), top(centred(e))
+        project = 2 + H * ir.dim ** 0.5
+        weigh = 100 * inner(dtype) * (top(v) * s).clamp_min(1.0)
+        error = {0: s * C * project * weigh, 1: s * s * ir.dim * (R * near_c + C * near_r + near_r * near_c) * (H + 2 * project) * weigh,
+                 3: s * R * project * weigh}
+        for k, allowed in error.items():
+            over = (got[k].cpu().double()[:, block] - want[k][:, block]).abs() / (step(dtype) * want[k][:, block].abs() + allowed + 2.0 ** -24 * (dtype == F16))
+            assert got[k].dtype == dtype and over.max().item() <= 1.0, f"{('gx', 'hx', 'hw', 'hg')[k]} of {mul}x{ir}: {over.max().item():.3g} of what is allowed"
+        # the weights': sums of s (P r) g over rows and components
+        allowed = (s * R * C * project * weigh).sum() * ir.dim
+        a, b = got[2].cpu()[channel:channel + mul], want[2][channel:channel + mul]
+        beyond = b.to(dtype).isinf()  # of the range of 16 bits
+        assert torch.equal(a[beyond], b.to(dtype)[beyond])
+        over = ((a.double() - b).abs() / (step(dtype) * b.abs() + allowed))[~beyond]
+        assert not over.numel() or over.max().item() <= 1.0, f"hw of {mul}x{ir}: {over.max().item():.3g} of what is allowed"
+        at, channel = at + mul * ir.dim, channel + mul
