@@ -218,13 +218,14 @@ def l0_feature_layout(specs) -> tuple[dict, int]:
 def edge_output_graph(graph: LunaTPGraph) -> LunaTPGraph:
     """The graph with the same sources in which edge ``e`` is destination ``e``: a convolution on it returns the
     messages themselves, one row per edge.  Built once per graph and kept with it."""
-    cached = graph._tables.get("edge_output_graph")
-    if cached is None:
+
+    def make():
         edges = graph.num_edges
         own = torch.arange(edges, device=graph.src.device, dtype=torch.int32)
-        cached = make_graph(graph.src, own, edges, num_src_nodes=graph.source_rows)
-        graph._tables["edge_output_graph"] = cached
-    return cached
+        found = make_graph(graph.src, own, edges, num_src_nodes=graph.source_rows)
+        return found, found.tensors()
+
+    return graph.derived("edge_output_graph", make)
 
 
 def create_uvu_conv_operator(official_tp_or_meta, *, dtype=None) -> LunaTPUVUConv:

@@ -10,6 +10,7 @@ that graphs can be prepared and inspected without a GPU.
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass, field
 from operator import index
 
@@ -37,6 +38,43 @@ class SourceSegmentTables:
     order: torch.Tensor
 
 
+# Held while tables are made on first use; one for all graphs, as that is rare.
+_making = threading.RLock()
+
+
+def _wait_for_tables(device: torch.device) -> None:
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+
+
+def _stream_in_use(device: torch.device):
+    return torch.cuda.current_stream(device) if device.type == "cuda" else None
+
+
+class _Derived:
+    """Tables that a graph makes on first use and keeps: ``value`` is what is asked for, ``tensors`` the memory it was made with.
+
+    No caller sees these tensors, so none can wait for them or keep their memory for a stream.  They are finished before anyone
+    finds them, and every stream that a call uses them on is recorded with them, so that their memory outlives its work.
+    """
+
+    __slots__ = ("value", "tensors", "streams")
+
+    def __init__(self, value, tensors):
+        self.value, self.tensors, self.streams = value, tensors, set()
+        if tensors:
+            _wait_for_tables(tensors[0].device)
+
+    def use(self):
+        if not torch.compiler.is_compiling():
+            stream = _stream_in_use(self.tensors[0].device)
+            if stream is not None and stream not in self.streams:
+                for tensor in self.tensors:
+                    tensor.record_stream(stream)
+                self.streams.add(stream)
+        return self.value
+
+
 class RowSplit:
     """One side (destinations or sources) of a graph whose long rows were cut into virtual rows.
 
@@ -57,6 +95,9 @@ class RowSplit:
         for j in range(1, int(pieces.max()) if degree.numel() else 1):
             nodes = torch.nonzero(pieces > j).squeeze(1)
             self.rounds.append((nodes, self.first[nodes] + j))
+
+    def tensors(self) -> list:
+        return [self.first, self.rows, *(t for pair in self.rounds for t in pair)]
 
     def gather(self, tensor: torch.Tensor | None) -> torch.Tensor | None:
         return None if tensor is None else tensor.index_select(0, self.rows)
@@ -88,6 +129,9 @@ class SplitGraph:
         self.graph = make_graph(src_virtual, dst_virtual, self.destinations.virtual_rows,
                                 num_src_nodes=self.sources.virtual_rows, split=False)
 
+    def tensors(self) -> list:
+        return self.destinations.tensors() + self.sources.tensors() + self.graph.tensors()
+
 
 @dataclass(frozen=True)
 class LunaTPGraph:
@@ -118,6 +162,26 @@ class LunaTPGraph:
     def source_rows(self) -> int:
         return self.num_nodes if self.num_src_nodes is None else int(self.num_src_nodes)
 
+    def derived(self, key, make):
+        """What ``make`` makes for this graph, once: it returns that and the tensors that were allocated for it (see ``_Derived``)."""
+        entry = self._tables.get(key)
+        if entry is None:
+            with _making:
+                entry = self._tables.get(key)
+                if entry is None:
+                    entry = _Derived(*make())
+                    self._tables[key] = entry
+        return entry.use() if entry.tensors else entry.value
+
+    def tensors(self) -> list:
+        """All tables."""
+        seg = self.source_segments
+        found = [self.src, self.dst, self.dst_rowptr, self.src_rowptr, self.edge_ids_by_src, self.edge_ids_by_dst, self.node_order,
+                 self.source_node_order, self.node_tiers]
+        if seg is not None:
+            found += [seg.nodes, seg.begin, seg.end, seg.rowptr, seg.order]
+        return [t for t in found if t is not None]
+
     def native(self) -> "_native.Graph":
         """The C-ABI view of this graph (cached; the tensors it points to are owned by the graph)."""
         view = self._tables.get("native")
@@ -144,17 +208,18 @@ class LunaTPGraph:
         A row of more than ``ROW_SPLIT_EDGES`` edges, or of half as many where that is four times the mean, would keep one
         multiprocessor busy when all others are done: such rows are cut into pieces of ``ROW_PIECE_EDGES``.  Decided once per
         graph (one read of the largest degree) and cached."""
-        holder = self._tables.get("rows")
-        if holder is None:
-            rowptr, pieces = self.dst_rowptr, [None] * 4
-            if self.can_split and self.num_edges:
-                degree = rowptr.diff()
-                longest = int(degree.max())
-                if longest > ROW_SPLIT_EDGES or longest > max(ROW_SPLIT_EDGES // 2, 4 * self.num_edges // self.num_nodes):
-                    limit = ROW_SPLIT_EDGES // 2
-                    rowptr, *pieces = _cut_rows(rowptr, degree, limit, ROW_PIECE_EDGES)
-            holder = self._tables["rows"] = _native.binding().Rows(rowptr, self.num_edges, *pieces)
-        return holder
+        return self.derived("rows", self._make_rows)
+
+    def _make_rows(self):
+        rowptr, pieces = self.dst_rowptr, []
+        if self.can_split and self.num_edges:
+            degree = rowptr.diff()
+            longest = int(degree.max())
+            if longest > ROW_SPLIT_EDGES or longest > max(ROW_SPLIT_EDGES // 2, 4 * self.num_edges // self.num_nodes):
+                limit = ROW_SPLIT_EDGES // 2
+                rowptr, *pieces = _cut_rows(rowptr, degree, limit, ROW_PIECE_EDGES)
+        holder = _native.binding().Rows(rowptr, self.num_edges, *(pieces or [None] * 4))
+        return holder, [rowptr, *pieces] if pieces else []
 
     def destination_range(self, begin: int, end: int) -> "tuple[LunaTPGraph, int, int]":
         """The graph of the edges whose destination lies in ``[begin, end)``, and that slice ``[e0, e1)`` of the edge
@@ -167,27 +232,26 @@ class LunaTPGraph:
         """
         if not 0 <= begin <= end <= self.num_nodes:
             raise ValueError(f"destination range [{begin}, {end}) outside [0, {self.num_nodes}]")
-        key = ("range", int(begin), int(end))
-        cached = self._tables.get(key)
-        if cached is None:
+
+        def make():
             e0, e1 = (int(v) for v in self.dst_rowptr[[begin, end]].tolist())
             piece = make_graph(self.src[e0:e1], self.dst[e0:e1] - begin, end - begin, num_src_nodes=self.source_rows)
-            cached = self._tables[key] = (piece, e0, e1)
-        return cached
+            return (piece, e0, e1), piece.tensors()
+
+        return self.derived(("range", int(begin), int(end)), make)
 
     def split_rows(self) -> "SplitGraph | None":
         """The virtual-row form of this graph if a node has more than ``ROW_SPLIT_EDGES`` edges on either side, else
         ``None``.  Decided once per graph (one read of the largest degree) and cached."""
-        try:
-            return self._tables["split"]
-        except KeyError:
-            split = None
-            if self.can_split and self.num_edges:
-                longest = int(torch.maximum(self.dst_rowptr.diff().max(), self.src_rowptr.diff().max()))
-                if longest > ROW_SPLIT_EDGES:
-                    split = SplitGraph(self, ROW_SPLIT_EDGES)
-            self._tables["split"] = split
-            return split
+        return self.derived("split", self._make_split)
+
+    def _make_split(self):
+        if self.can_split and self.num_edges:
+            longest = int(torch.maximum(self.dst_rowptr.diff().max(), self.src_rowptr.diff().max()))
+            if longest > ROW_SPLIT_EDGES:
+                split = SplitGraph(self, ROW_SPLIT_EDGES)
+                return split, split.tensors()
+        return None, []
 
     def table_list(self) -> list:
         """The 13 tensors the reference passes to its custom ops (``src/lunatp/uvu_conv/interface.py:186-192``)."""

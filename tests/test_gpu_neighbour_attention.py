@@ -201,3 +201,42 @@ def test_second_order_of_the_layer_norm_far_from_zero(irreps, rows, dtype, shift
         over = ((a.double() - b).abs() / (step(dtype) * b.abs() + allowed))[~beyond]
         assert not over.numel() or over.max().item() <= 1.0, f"hw of {mul}x{ir}: {over.max().item():.3g} of what is allowed"
         at, channel = at + mul * ir.dim, channel + mul
+
+
+def test_first_calls_of_two_streams():
+    """The tables of cut rows are made in the first call; one on another stream right behind it finds them finished."""
+    generator = torch.Generator().manual_seed(0)
+    dst = torch.repeat_interleave(torch.arange(300), torch.tensor(([3] * 99 + [3000]) * 3)).to(DEVICE)
+    z = torch.randn(dst.numel(), 2, generator=generator).to(DEVICE)
+    want = luna.graph_softmax(z, luna.make_graph(torch.zeros_like(dst), dst, 300))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        graph = luna.make_graph(torch.zeros_like(dst), dst, 300)
+        torch.cuda.synchronize()
+        found = []
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                found.append(luna.graph_softmax(z, graph))
+        torch.cuda.synchronize()
+        assert all(torch.equal(f, want) for f in found)
+
+
+def test_tables_outlive_the_work_of_other_streams():
+    """Memory of tables that no caller sees is not handed out again while a stream that they were used on is busy."""
+    dst = torch.repeat_interleave(torch.arange(300), torch.tensor(([3] * 99 + [3000]) * 3)).to(DEVICE)
+    z = torch.randn(dst.numel(), 2, device=DEVICE)
+    graph = luna.make_graph(torch.zeros_like(dst), dst, 300)
+    want = luna.graph_softmax(z, graph)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # a fifth of a second
+        got = luna.graph_softmax(z, graph)
+    tables = graph._tables["rows"].tensors
+    places, sizes = {t.data_ptr() for t in tables}, [t.numel() for t in tables]
+    del graph, tables
+    again = [torch.empty(n, dtype=torch.int32, device=DEVICE) for n in sizes for _ in range(4)]
+    assert not side.query()  # still asleep
+    assert not places & {t.data_ptr() for t in again}
+    side.synchronize()
+    assert torch.equal(got, want)

@@ -1,9 +1,15 @@
 """What the operators of attention over neighbours do on the host: checks at the entry points, and tables that are made once."""
 
 import ctypes
+import threading
 
+import pytest
+import torch
 
+import lunaequivariance_b200 as luna
 from lunaequivariance_b200 import _native
+from lunaequivariance_b200 import graph as graph_mod
+from lunaequivariance_b200.conv import edge_output_graph
 
 
 def test_wide_cotangents_are_checked():
@@ -27,3 +33,79 @@ def test_wide_cotangents_are_checked():
         assert second(dtype) == second(dtype, alpha=None, g=some) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert backward(9) == second(9) == _native.LUNA_ERR_INVALID_ARGUMENT
     assert backward(_native.LUNA_F32, g=ctypes.c_void_p(18)) == _native.LUNA_ERR_MISALIGNED
+
+
+def hub_graph(monkeypatch):
+    monkeypatch.setattr(graph_mod, "ROW_SPLIT_EDGES", 8)
+    monkeypatch.setattr(graph_mod, "ROW_PIECE_EDGES", 4)
+    dst = torch.repeat_interleave(torch.arange(5), torch.tensor([3, 20, 0, 9, 30]))
+    return luna.make_graph(torch.randint(5, dst.shape, generator=torch.Generator().manual_seed(0)), dst, 5)
+
+
+# What a graph makes on first use, by the name it is kept under.
+DERIVED = {"rows": lambda g: g.row_holder(), "split": lambda g: g.split_rows(), ("range", 1, 4): lambda g: g.destination_range(1, 4),
+           "edge_output_graph": edge_output_graph}
+
+
+@pytest.mark.parametrize("name", list(DERIVED), ids=str)
+def test_tables_are_finished_before_anyone_finds_them(name, monkeypatch):
+    """Another stream's or thread's call takes what is kept at once: it is kept only after the stream that makes it was waited for."""
+    graph, waits = hub_graph(monkeypatch), []
+
+    def wait(device):
+        assert name not in graph._tables
+        waits.append(device)
+
+    monkeypatch.setattr(graph_mod, "_wait_for_tables", wait)
+    first = DERIVED[name](graph)
+    assert waits == [graph.src.device] and name in graph._tables
+    assert DERIVED[name](graph) is first and len(waits) == 1
+
+
+@pytest.mark.parametrize("name", list(DERIVED), ids=str)
+def test_tables_are_made_once_for_two_threads(name, monkeypatch):
+    graph, begun, finished, waits = hub_graph(monkeypatch), threading.Event(), threading.Event(), []
+
+    def wait(device):
+        waits.append(device)
+        begun.set()
+        assert finished.wait(20)
+
+    monkeypatch.setattr(graph_mod, "_wait_for_tables", wait)
+    found = [None, None]
+
+    def call(i):
+        found[i] = DERIVED[name](graph)
+
+    threads = [threading.Thread(target=call, args=(i,), daemon=True) for i in range(2)]
+    threads[0].start()
+    assert begun.wait(20)
+    threads[1].start()
+    threads[1].join(0.2)
+    assert found == [None, None]  # neither has tables that are not finished
+    finished.set()
+    for thread in threads:
+        thread.join(20)
+    assert found[0] is not None and found[0] is found[1] and len(waits) == 1
+
+
+@pytest.mark.parametrize("name", list(DERIVED), ids=str)
+def test_memory_of_tables_is_kept_for_every_stream(name, monkeypatch):
+    """Tables that no caller sees are recorded once with each stream that a call uses them on."""
+    graph, recorded = hub_graph(monkeypatch), []
+    stream = None
+    monkeypatch.setattr(graph_mod, "_stream_in_use", lambda device: stream)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: recorded.append((t.data_ptr(), s)))
+    for stream in ("one", "other", "one", "other"):
+        DERIVED[name](graph)
+    tables = {t.data_ptr() for t in graph._tables[name].tensors}
+    assert sorted(recorded) == sorted((t, s) for s in ("one", "other") for t in [t.data_ptr() for t in graph._tables[name].tensors])
+    own = {t.data_ptr() for t in graph.tensors() if t.numel()}
+    assert len(tables) > 1 and not tables & own
+
+
+def test_graphs_without_tables_of_their_own_wait_for_nothing(monkeypatch):
+    monkeypatch.setattr(graph_mod, "_wait_for_tables", lambda device: pytest.fail("waited"))
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: pytest.fail("recorded"))
+    graph = luna.make_graph(torch.tensor([0, 1, 1]), torch.tensor([0, 1, 1]), 2)
+    assert graph.split_rows() is None and graph.row_holder() is graph.row_holder()
