@@ -9,8 +9,10 @@ from __future__ import annotations
 from collections.abc import Mapping
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
+from torch._subclasses.functional_tensor import FunctionalTensor
 
-from .conv import create_uvu_conv_operator
+from .conv import create_uvu_conv_operator, is_compiling
 from .functional import require_uvu, resolve_source, tensor_product, tensor_product_conv
 from .graph import make_graph
 from .layer_norm import LayerNormConfig, layer_norm
@@ -257,21 +259,37 @@ class RelativeBias(torch.nn.Module):
         if heads < 1:
             raise ValueError("RelativeBias needs a positive number of heads")
         self.weight = torch.nn.Parameter(torch.zeros(len(self._boundaries) + 1, heads, device=device, dtype=dtype))
-        self._borders = {}
+        self._make_borders()
 
     boundaries = property(lambda self: self._boundaries)
 
     def _apply(self, fn, recurse=True):
         result = super()._apply(fn, recurse=recurse)
-        self._borders = {}
+        self._make_borders()
         return result
+
+    def _make_borders(self):
+        # Beside the weights, for vectors of either type: a program that is compiled or captured finds them there.
+        self._borders = {}
+        for dtype in (torch.float32, torch.float64):
+            self._keep_borders(self.weight.device, dtype)
+
+    def _keep_borders(self, device, dtype):
+        with torch.inference_mode(False):
+            borders = torch.tensor(self._boundaries, device=device, dtype=dtype)
+        if type(borders) is torch.Tensor:  # not a stand-in of a trace, which has no numbers and is of no use behind it
+            self._borders[device, dtype] = borders
+        return borders
 
     def buckets(self, vec):
         """The bucket of every vector ``vec[..., 3]``, whatever the type of the weights."""
-        key = (vec.device, vec.dtype)
-        borders = self._borders.get(key)
+        # A trace with stand-ins for tensors takes the borders as constants of its own.
+        borders = None if isinstance(vec, (FakeTensor, FunctionalTensor)) else self._borders.get((vec.device, vec.dtype))
         if borders is None:
-            borders = self._borders[key] = torch.tensor(self._boundaries, device=vec.device, dtype=vec.dtype)
+            if is_compiling():
+                borders = torch.tensor(self._boundaries, device=vec.device, dtype=vec.dtype)
+            else:
+                borders = self._keep_borders(vec.device, vec.dtype)
         return distance_buckets(vec, borders)
 
     def forward(self, vec):

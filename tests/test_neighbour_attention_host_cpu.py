@@ -109,3 +109,39 @@ def test_graphs_without_tables_of_their_own_wait_for_nothing(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: pytest.fail("recorded"))
     graph = luna.make_graph(torch.tensor([0, 1, 1]), torch.tensor([0, 1, 1]), 2)
     assert graph.split_rows() is None and graph.row_holder() is graph.row_holder()
+
+
+@pytest.mark.parametrize("known", [True, False])
+def test_a_trace_leaves_no_stand_ins_in_a_module(known):
+    """Borders of a trace with stand-ins for tensors stay in it: the next trace, and calls with numbers, have their own."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    module = luna.RelativeBias([1.0, 2.5], 3)
+    if not known:
+        module._borders = {}
+    before = set(module._borders)
+    for mode in ("fake", "symbolic", "fake"):
+        traced = make_fx(lambda v: module.buckets(v), tracing_mode=mode)(torch.randn(5, 3))
+        assert traced._tensor_constant0.shape == (2,)
+        assert set(module._borders) == before
+    exported = torch.export.export(_Buckets(module), (torch.randn(5, 3),), strict=False)
+    assert "lunaeq.distance_buckets" in str(exported.graph) and set(module._borders) == before
+    with torch._subclasses.fake_tensor.FakeTensorMode():
+        assert luna.RelativeBias([1.0], 2)._borders == {}
+    with torch.inference_mode():
+        assert not any(t.is_inference() for t in luna.RelativeBias([1.0], 2)._borders.values())
+    for dtype in (torch.float32, torch.float64):
+        with pytest.raises(RuntimeError, match="CUDA is required"):  # in the launch, with what is kept for it
+            module.buckets(torch.zeros(1, 3, dtype=dtype))
+        kept = module._borders[torch.device("cpu"), dtype]
+        assert type(kept) is torch.Tensor and kept.dtype == dtype and kept.tolist() == [1.0, 2.5]
+    assert all(t.dtype in (torch.float32, torch.float64) for t in module.half()._borders.values()) and len(module._borders) == 2
+
+
+class _Buckets(torch.nn.Module):
+    def __init__(self, module):
+        super().__init__()
+        self.module = module
+
+    def forward(self, vec):
+        return self.module.buckets(vec)
