@@ -135,9 +135,12 @@ struct Place {
   }
 
   // Starts the copies of a round of rows, of which `row` is this team's, from arrays of P.rows rows.  Rounds are asked for in order.
+  // They refill what has been read before.  A copy is ordered with the thread's own reads by a barrier, not by standing behind
+  // them: that of the warp for packets, which costs nothing that could be measured, that of the CTA, which is there, for chunks.
   __device__ __forceinline__ void request(const Params& P, const T* const (&arrays)[IN], int64_t row) {
     if (MODE == kDirect) return;
     if (MODE == kPackets) {
+      __syncwarp();
 #pragma unroll
       for (int a = 0; a < IN; ++a) {
         if (!arrays[a]) continue;
@@ -342,7 +345,7 @@ __device__ __forceinline__ void forward(const Params& P, const Block& B, int ind
 #pragma unroll
       for (int c = 0; c < VEC; ++c) sums[0] += v[k][c] * v[k][c];
     place.sum(sums);
-    if (MODE == kPackets) request(row + kStages * step);  // the thread's numbers of this row have gone into the sum
+    if (MODE == kPackets) request(row + kStages * step);  // the thread's numbers of this row are in registers
     const A scale = rsqrt(sums[0] * share + eps);
 #pragma unroll
     for (int k = 0; k < K; ++k)

@@ -240,3 +240,17 @@ def test_tables_outlive_the_work_of_other_streams():
     assert not places & {t.data_ptr() for t in again}
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64, BF16])
+@pytest.mark.parametrize("irreps,rows", [(4, 300_001), (64, 60_000), ("16x0e+16x1o", 40_000), (1024, 5000)])
+def test_packets_are_read_before_they_are_refilled(irreps, rows, dtype):
+    """The gradient of the weights alone asks for the next rows right behind its reads: the same bits as beside the rows' gradient."""
+    config = luna.LayerNormConfig(irreps)
+    generator = torch.Generator(device=DEVICE).manual_seed(0)
+    x, g = (torch.randn(rows, config.dim, generator=generator, device=DEVICE).to(dtype).requires_grad_(True) for _ in range(2))
+    w = torch.rand(config.weight_numel, generator=generator, device=DEVICE).to(dtype).requires_grad_(True)
+    _, both = torch.autograd.grad(luna.layer_norm(x, config.irreps, w), (x, w), g)
+    for _ in range(20):
+        alone, = torch.autograd.grad(luna.layer_norm(x.detach(), config.irreps, w), w, g)
+        assert torch.equal(alone, both)
