@@ -785,7 +785,8 @@ int64_t bytes_of(const Tensor& t) { return t.defined() ? t.numel() : 0; }
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------------
 struct Norm : torch::CustomClassHolder {
-  luna_norm_desc desc{};  // the type comes with each call
+  static constexpr int64_t kMostElements = 16384;  // of a block
+  luna_norm_desc desc{};                           // the type comes with each call
   int64_t dim = 0, weights = 0, biases = 0;
   Norm(const std::vector<std::array<int64_t, 3>>& blocks, int64_t normalization, double eps) {
     TORCH_CHECK_NOT_IMPLEMENTED(blocks.size() <= 32, "layer norm of more than 32 blocks");
@@ -794,6 +795,8 @@ struct Norm : torch::CustomClassHolder {
     desc.eps = eps;
     for (size_t i = 0; i < blocks.size(); ++i) {
       const auto& [mul, components, scalar] = blocks[i];
+      TORCH_CHECK_NOT_IMPLEMENTED(mul <= kMostElements && components <= kMostElements, "layer norm of a block with more than ", kMostElements,
+                                  " elements");  // also beyond what the description holds
       desc.mul[i] = static_cast<int32_t>(mul);
       desc.components[i] = static_cast<int32_t>(components);
       desc.scalar[i] = static_cast<int32_t>(scalar);

@@ -254,3 +254,26 @@ def test_packets_are_read_before_they_are_refilled(irreps, rows, dtype):
     for _ in range(20):
         alone, = torch.autograd.grad(luna.layer_norm(x.detach(), config.irreps, w), w, g)
         assert torch.equal(alone, both)
+
+
+def test_borders_are_there_before_the_first_call():
+    """A module that is captured, or compiled, before it has ever been called."""
+    module = luna.RelativeBias([0.5, 1.0, 2.0], 4, device=DEVICE)
+    with torch.no_grad():
+        module.weight.normal_()
+    vec = torch.randn(50, 3, device=DEVICE)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        luna.distance_buckets(vec, torch.zeros(1, device=DEVICE))
+    torch.cuda.current_stream().wait_stream(side)
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        found = module.buckets(vec)
+    captured.replay()
+    want = oracle.distance_buckets(vec.cpu(), torch.tensor([0.5, 1.0, 2.0]))
+    assert torch.equal(found.cpu(), want)
+    fresh = luna.RelativeBias([0.5, 1.0, 2.0], 4, device=DEVICE)
+    fresh._borders = {}
+    assert torch.equal(torch.compile(lambda v: fresh.buckets(v), fullgraph=True)(vec).cpu(), want)
+    assert not fresh._borders and torch.equal(fresh.buckets(vec).cpu(), want)

@@ -145,3 +145,10 @@ class _Buckets(torch.nn.Module):
 
     def forward(self, vec):
         return self.module.buckets(vec)
+
+
+def test_sizes_beyond_the_description():
+    """Blocks that a description of 32 bits would hold as others are refused like all that are too long."""
+    for irreps in (16385, "1x0e+20000x1o", (1 << 32) + 64):
+        with pytest.raises(NotImplementedError, match="16384"):
+            luna.LayerNormConfig(irreps).holder()
