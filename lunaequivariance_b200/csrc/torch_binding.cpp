@@ -825,6 +825,13 @@ luna_norm_desc check_norm(const Norm& n, const Tensor& x, const Tensor& weight, 
   return desc;
 }
 
+// The statistics as a forward leaves them: the launches follow them by the sizes of x.
+Tensor check_stats(const Norm& n, const Tensor& x, const Tensor& stats) {
+  TORCH_CHECK_VALUE(stats.defined(), "layer norm needs the forward's statistics");
+  check_beside(x, stats, "stats", {n.desc.num_blocks, x.numel() / n.dim, 2}, x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat);
+  return prepared(stats);
+}
+
 std::array<Tensor, 2> norm_forward(const Norm& n, const Tensor& x, const Tensor& weight, const Tensor& bias, bool keep_stats) {
   const luna_norm_desc desc = check_norm(n, x, weight, bias);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -844,12 +851,12 @@ std::array<Tensor, 3> norm_backward(const Norm& n, const Tensor& x, const Tensor
   refuse_tangents({&g});
   check_beside(x, g, "grad_out", x.sizes());
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = norm_rows(x, n), w = contiguous(weight), cotangents = norm_rows(g, n);
+  const Tensor rows = norm_rows(x, n), w = contiguous(weight), cotangents = norm_rows(g, n), moments = check_stats(n, x, stats);
   if (mask & 1) out[0] = at::empty(x.sizes(), rows.options());
   if (mask & 2) out[1] = at::empty({n.weights}, rows.options());
   if (mask & 4) out[2] = at::empty({n.biases}, rows.options());
   const Tensor scratch = mask & 6 ? scratch_of(api.norm_scratch_bytes(&desc, rows.size(0)), x) : Tensor();
-  check(api.norm_bwd(&desc, rows.data_ptr(), pointer(w), stats.data_ptr(), cotangents.data_ptr(), pointer(out[0]), pointer(out[1]),
+  check(api.norm_bwd(&desc, rows.data_ptr(), pointer(w), moments.data_ptr(), cotangents.data_ptr(), pointer(out[0]), pointer(out[1]),
                      n.biases ? pointer(out[2]) : nullptr, pointer(scratch), bytes_of(scratch), rows.size(0), stream_of(x)));
   return out;
 }
@@ -867,12 +874,12 @@ std::array<Tensor, 3> norm_double(const Norm& n, const Tensor& x, const Tensor& 
   check_beside(x, rb, "rb", {n.biases});
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor rows = norm_rows(x, n), w = contiguous(weight), cotangents = norm_rows(g, n), tx = norm_rows(rx, n), tw = contiguous(rw),
-               tb = contiguous(rb);
+               tb = contiguous(rb), moments = check_stats(n, x, stats);
   if (mask & 1) out[0] = at::empty(x.sizes(), rows.options());
   if (mask & 2) out[1] = at::empty({n.weights}, rows.options());
   if (mask & 4) out[2] = at::empty(x.sizes(), rows.options());
   const Tensor scratch = mask & 2 ? scratch_of(api.norm_scratch_bytes(&desc, rows.size(0)), x) : Tensor();
-  check(api.norm_dbl_bwd(&desc, rows.data_ptr(), pointer(w), stats.data_ptr(), cotangents.data_ptr(), pointer(tx), pointer(tw),
+  check(api.norm_dbl_bwd(&desc, rows.data_ptr(), pointer(w), moments.data_ptr(), cotangents.data_ptr(), pointer(tx), pointer(tw),
                          n.biases ? pointer(tb) : nullptr, pointer(out[0]), pointer(out[1]), pointer(out[2]), pointer(scratch),
                          bytes_of(scratch), rows.size(0), stream_of(x)));
   return out;
@@ -1056,6 +1063,9 @@ struct Rows : torch::CustomClassHolder {
   Rows(const Tensor& rowptr, int64_t edges, const Maybe& piece_of_row, const Maybe& row_of_piece, const Maybe& cut_of_piece,
        const Maybe& cut_first)
       : tables{rowptr, of(piece_of_row), of(row_of_piece), of(cut_of_piece), of(cut_first)} {
+    for (const Tensor& t : tables)
+      TORCH_CHECK_VALUE(!t.defined() || (t.dim() == 1 && t.is_contiguous()), "tables of rows must be one-dimensional and contiguous, got ", t.sizes());
+    TORCH_CHECK_VALUE(rowptr.numel() > 0, "row pointers must not be empty");
     native.num_rows = rowptr.numel() - 1;
     native.num_edges = edges;
     native.rowptr = rowptr.data_ptr<int32_t>();

@@ -256,6 +256,23 @@ def test_packets_are_read_before_they_are_refilled(irreps, rows, dtype):
         assert torch.equal(alone, both)
 
 
+def test_statistics_of_another_call_are_refused():
+    """The operators behind the layer norm take the forward's statistics as an argument, and follow them by the sizes of the rows."""
+    ops, config = torch.ops.lunaeq, luna.LayerNormConfig("8x0e+4x1o").descriptor()
+    x, g = torch.randn(6, 20, device=DEVICE), torch.randn(6, 20, device=DEVICE)
+    stats = ops.layer_norm_forward(x, None, None, config)[1]
+    assert stats.shape == (2, 6, 2)
+    needs = [True, False, False]
+    want = ops.layer_norm_backward(x, None, stats, g, needs, config)[0]
+    # in another order of memory they are what they were
+    assert torch.equal(ops.layer_norm_backward(x, None, stats.permute(2, 1, 0).contiguous().permute(2, 1, 0), g, needs, config)[0], want)
+    for bad, error in ((stats[:, :3], ValueError), (stats[:1], ValueError), (stats.flatten(), ValueError), (stats.double(), TypeError), (stats.cpu(), ValueError)):
+        with pytest.raises(error, match="stats"):
+            ops.layer_norm_backward(x, None, bad, g, needs, config)
+        with pytest.raises(error, match="stats"):
+            ops.layer_norm_double_backward(x, None, bad, g, x, None, None, needs, config)
+
+
 def test_borders_are_there_before_the_first_call():
     """A module that is captured, or compiled, before it has ever been called."""
     module = luna.RelativeBias([0.5, 1.0, 2.0], 4, device=DEVICE)

@@ -152,3 +152,15 @@ def test_sizes_beyond_the_description():
     for irreps in (16385, "1x0e+20000x1o", (1 << 32) + 64):
         with pytest.raises(NotImplementedError, match="16384"):
             luna.LayerNormConfig(irreps).holder()
+
+
+def test_tables_of_rows_that_launches_could_not_follow():
+    rows = _native.binding().Rows
+    numbers = torch.arange(8, dtype=torch.int32)
+    for bad in (numbers[::2], numbers.reshape(2, 4), numbers[:0]):
+        with pytest.raises(ValueError, match="row"):
+            rows(bad, 4, None, None, None, None)
+    with pytest.raises(ValueError, match="rows"):
+        rows(numbers, 4, numbers[::2], numbers, numbers, numbers)
+    with pytest.raises(RuntimeError, match="Int"):
+        rows(numbers.long(), 4, None, None, None, None)
