@@ -294,3 +294,41 @@ def test_borders_are_there_before_the_first_call():
     fresh._borders = {}
     assert torch.equal(torch.compile(lambda v: fresh.buckets(v), fullgraph=True)(vec).cpu(), want)
     assert not fresh._borders and torch.equal(fresh.buckets(vec).cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F64, BF16, F16])
+@pytest.mark.parametrize("edges,buckets,heads", [(600_007, 128, 16), (900_001, 64, 8), (400_003, 32, 1), (700_009, 25, 3), (300_013, 16, 33),
+                                                 (200_003, 5000, 12), (150_001, 7, 130), (1_000_003, 2, 4)])
+def test_sums_by_bucket_of_many_runs(edges, buckets, heads, dtype):
+    """Whole numbers that differ from edge to edge, in tens of runs of each copy of the table: their sums are exact, however they are made."""
+    generator = torch.Generator(device=DEVICE).manual_seed(edges)
+    g = torch.randint(-8, 9, (edges, heads), generator=generator, device=DEVICE).to(dtype)
+    index = torch.randint(-1, buckets + 1, (edges + 1,), generator=generator, device=DEVICE, dtype=torch.int32)
+    index[: edges // 3] = index[: edges // 3].sort()[0]  # long stretches of one bucket, then none
+    table = torch.zeros(buckets, heads, device=DEVICE, dtype=dtype, requires_grad=True)
+    for those in (index[:-1], index[1:]):  # aligned to whole packets and not
+        got, = torch.autograd.grad(luna.relative_bias(table, those), table, g)
+        inside = (those >= 0) & (those < buckets)
+        sums = torch.zeros(buckets, heads, dtype=F64, device=DEVICE).index_add_(0, those[inside].long(), g[inside].double())
+        assert sums.abs().max() < 2 ** 24 and torch.equal(got, sums.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, F64, BF16])
+def test_sums_by_bucket_behind_a_softmax_of_many_edges(dtype):
+    """The table's gradient, bucket by bucket: the parts' errors as in the tests above, and 300 additions one after the other."""
+    nodes, degree, heads, buckets = 8000, 50, 8, 64
+    generator = torch.Generator(device=DEVICE).manual_seed(0)
+    rand = lambda *shape: torch.randn(*shape, generator=generator, device=DEVICE).to(dtype)  # noqa: E731
+    dst = torch.arange(nodes, device=DEVICE).repeat_interleave(degree)
+    z, t, g = rand(nodes * degree, heads), rand(buckets, heads), rand(nodes * degree, heads)
+    index = torch.randint(buckets, (nodes * degree,), generator=generator, device=DEVICE, dtype=torch.int32)
+    leaf = t.clone().requires_grad_(True)
+    got, = torch.autograd.grad(luna.graph_softmax(z, luna.make_graph(dst, dst, nodes), table=leaf, buckets=index), leaf, g)
+    alpha = (z.double() + t.double()[index.long()]).reshape(nodes, degree, heads).softmax(1)
+    e = g.double().reshape(nodes, degree, heads)
+    gz = (alpha * (e - (alpha * e).sum(1, keepdim=True))).reshape(-1, heads)
+    want = torch.zeros(buckets, heads, dtype=F64, device=DEVICE).index_add_(0, index.long(), gz)
+    relative = inner(dtype) * (4 * (z.double().abs().max() + t.double().abs().max()) + 64 + 30)
+    parts = 4 * relative * alpha.reshape(-1, heads) * e.abs().max() + 300 * inner(dtype) * gz.abs()
+    allowed = torch.zeros_like(want).index_add_(0, index.long(), parts) + step(dtype) * want.abs()
+    assert ((got.double() - want).abs() <= allowed).all()
