@@ -65,6 +65,9 @@ class _Derived:
         if tensors:
             _wait_for_tables(tensors[0].device)
 
+    def __reduce__(self):  # a copy has memory of its own, which no stream has used
+        return _Derived, (self.value, self.tensors)
+
     def use(self):
         if not torch.compiler.is_compiling():
             stream = _stream_in_use(self.tensors[0].device)

@@ -164,3 +164,18 @@ def test_tables_of_rows_that_launches_could_not_follow():
         rows(numbers, 4, numbers[::2], numbers, numbers, numbers)
     with pytest.raises(RuntimeError, match="Int"):
         rows(numbers.long(), 4, None, None, None, None)
+
+
+@pytest.mark.parametrize("name", ["split", ("range", 1, 4), "edge_output_graph"], ids=str)
+def test_graphs_are_copied_with_their_tables(name, monkeypatch):
+    import copy
+    import pickle
+
+    graph = hub_graph(monkeypatch)
+    monkeypatch.setattr(graph_mod, "_stream_in_use", lambda device: lambda: None)  # no stream can be copied
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: None)
+    DERIVED[name](graph)
+    for other in (copy.deepcopy(graph), pickle.loads(pickle.dumps(graph))):
+        mine, its = graph._tables[name].tensors, other._tables[name].tensors
+        assert len(mine) == len(its) and all(torch.equal(a, b) and a.data_ptr() != b.data_ptr() for a, b in zip(mine, its) if a.numel())
+        assert not other._tables[name].streams
