@@ -256,7 +256,8 @@ LUNA_API int luna_sh_dbl_bwd(const luna_sh_desc* desc, const void* v, const void
  * sqrt(share * sum of squares + eps) with share = 1/(mul*components) (normalization 0, "component") or 1/mul (1, "norm"),
  * then multiplied by one weight per channel, and scalars get one bias per channel.  weight[sum of mul] and bias[sum of mul
  * of the scalar blocks] are consecutive in block order; null means ones and zeros.  At most 32 blocks of at most 16384
- * elements (LUNA_ERR_UNSUPPORTED beyond).  Sums are held in float (double for LUNA_F64), without atomics: the same call gives the same bits.
+ * elements (LUNA_ERR_UNSUPPORTED beyond).  Sums are held in float (double for LUNA_F64), without atomics: the same sizes on the same
+ * device, in arrays of the same alignment, give the same bits (how rows are cut up depends on these).
  *
  * stats: what the forward leaves for the others, rows * num_blocks pairs (mean, scale) of float or double, in block-major
  * order; the forward skips it if null. */
@@ -284,7 +285,7 @@ LUNA_API int luna_layer_norm_dbl_bwd(const luna_norm_desc* desc, const void* x, 
  * double precision; boundaries ascending and not negative), for v[n,3] of LUNA_F32 or LUNA_F64.
  * luna_relative_bias_fwd: out[edges, heads] = table[buckets[e], heads]; an edge whose bucket is no row of the table gets
  * zeros.  luna_relative_bias_bwd: gtable[num_buckets, heads] = sums of g over the edges of each bucket, without atomics,
- * in an order that depends on the sizes alone. */
+ * in an order that depends on the sizes, the alignment of g and the device. */
 LUNA_API int luna_distance_buckets(int dtype, const void* v, const void* boundaries, int64_t num_boundaries, int32_t* out,
                                    int64_t n, void* stream);
 LUNA_API int luna_relative_bias_fwd(int dtype, const void* table, const int32_t* buckets, void* out, int64_t edges,

@@ -108,7 +108,8 @@ struct Together {
 };
 
 // exp(z - m), in single precision as 2^((z - m) log2 e): a product, rounded once, and an instruction that is off by two units in
-// the last place.  The difference is made first: z and m may be the lowest numbers of their type.
+// the last place.  So the result is off by |z - m| roundings of 2^-24 and a few (a millionth at 20 below the largest), and below 1.2e-38
+// it is zero.  The difference is made first: z and m may be the lowest numbers of their type.
 __device__ __forceinline__ float exponential(float z, float m) {
   float v;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"((z - m) * 1.4426950408889634f));
@@ -447,14 +448,19 @@ int start(const Rows& R, const Shape& S, const Operands<T>& o, Pair<Acc<T>>* sta
 template <typename T, int VEC, int ORDER>
 int launch(const Rows& R, int64_t edges, int64_t heads, int64_t num_buckets, const Operands<T>& o, void* scratch, cudaStream_t stream) {
   // Sixteen numbers of a thread in registers; single ones, with their exponentials and addresses, spill (forward, 2.6 M edges
-  // with one head: 23 us, with eight 14; the backward has room: 8.3 and 9.8).
+  // with one head: 23 us, with eight 14; the backward has room: 8.3 and 9.8).  Pairs spill, too (90 to 130 bytes), and of
+  // sixteen and eight either is faster somewhere: FP32, us, forward without and with bias and mask, second order: two heads 23 / 41 / 32
+  // and 27 / 38 / 34, six 47 / 77 / 66 and 50 / 64 / 80.
   constexpr int K = sizeof(T) > 4 ? 8 / VEC : VEC == 1 && !is_backward(ORDER) ? 8 : 16 / VEC;
   Shape S{};
   S.heads = static_cast<int>(heads);
   S.num_buckets = static_cast<int>(num_buckets);
   const int64_t packets = heads / VEC;
   S.across = packets >= 32 ? 32 : rows::next_power_of_two(packets);
-  // As many threads as hold a row (of the pieces, one) somewhat longer than the mean; a CTA where a warp would read most of a row twice.
+  // As many threads as hold a row (of the pieces, one) somewhat longer than the mean; a CTA where a warp would read most of a row twice:
+  // four times what it holds.  2.6 M edges of 8 heads, FP32, in rows of 200, 250, 300, 400 and 500, by a warp or a CTA, us: forward 40,
+  // 38, 41, 41, 45 or 88, 74, 65, 54, 49; backward 52, 57, 57, 60, 68 or 64, 56, 52, 48, 47.  It is the backward that changes sides where
+  // the rule does (at 205 edges).
   const int64_t mean = ceil_div(edges, R.count);
   const int64_t wanted = ceil_div(mean + mean / 4, K) * S.across;
   S.lanes = wanted > 128 ? kThreads : wanted >= 32 ? 32 : rows::next_power_of_two(wanted);

@@ -12,7 +12,7 @@
 // is normalised alone, so a CTA works on one block's columns of many rows: `lanes` threads (a power of two; up to a whole
 // CTA) share a row, each with up to K packets of VEC elements, always the same columns, so that it keeps their weights and
 // the sums of the weights' gradients in registers from row to row.  Those sums meet once per CTA and once more in a second
-// launch, in an order that only the sizes decide: no atomics, the same bits every time.
+// launch, without atomics, in an order that the sizes, the alignment of the arrays and the device decide: the same call gives the same bits.
 //
 // Rows arrive in shared memory by asynchronous copies, one round ahead of their use, so that the memory is busy while sums
 // are made.  Each thread copies what it will read itself, in the widest packets that the rows allow, and waits for nobody.  16-bit
@@ -658,7 +658,7 @@ int launch(Params P, const Call& c, cudaStream_t stream) {
 
 // Packets narrower than sixteen bytes.  Numbers of a thread, measured, forward / backward in us for four, eight or sixteen: 600,000 rows
 // of 50x0e, FP32 (packets of two) 55 / 78, 43 / 72, 46 / 76, BF16 56 / 80, 41 / 67, 37 / 59; 20,000 of 1001x0e, FP32 (single numbers)
-// 55 / 64, 39 / 67, 44 / 72; 300,000 of 51x0e, FP64, four or eight 44 / 69 / 110 (second order) and 48 / 75 / 159.
+// 55 / 64, 39 / 67, 44 / 72; 300,000 of 51x0e, FP64, four or eight 44 / 69 / 112 (second order) and 48 / 75 / 180.
 template <typename T, int VEC, int ORDER>
 int with_packets(const Params& P, int64_t longest, bool few, const Call& c, cudaStream_t stream) {
   constexpr int kFew = VEC < 4 ? 4 / VEC : 1, kMany = (sizeof(T) == 2 && ORDER != kSecond ? 16 : 8) / VEC;
@@ -682,7 +682,7 @@ int choose(const Params& P, const Call& c, cudaStream_t stream) {
     while (vec > 1 && !aligned_to(p, vec * sizeof(T))) vec >>= 1;
   // Packets of a thread.  More of them mean fewer threads per row, so fewer steps for its sums and no barrier, as long as the
   // registers allow it.  Measured, forward / backward / second order in us: 50,000 rows of 128x0e+128x1o+128x2e, FP32, one, two
-  // or four packets 139 / 199, 87 / 168, 84 / 123; 100,000 of 64x0e+64x1o+64x2e 139 / 180 / 336, 86 / 163 / 235, 82 / 123 / 287;
+  // or four packets 139 / 199, 87 / 168, 84 / 123; 100,000 of 64x0e+64x1o+64x2e 139 / 180 / 316, 86 / 163 / 244, 82 / 123 / 308;
   // 86,000 of 64x0e 10.9 / 13.0, 8.9 / 14.9, 9.7 / 15.4; 40,000 of 1024x0e, BF16, 58 / 76, 55 / 63, 54 / 79.  Where there are not
   // enough rows to fill the GPU, the threads are: 24 rows 2.6, 2.8 and 3.6 us, 500 rows of 64x0e 2.6 / 3.1, 3.1 / 4.2, 4.0 / 5.7.
   const bool few = P.rows * P.dim <= static_cast<int64_t>(rows::processors()) * 1024 * (vec == kWidest ? kWidest : 1);

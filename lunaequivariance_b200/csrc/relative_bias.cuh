@@ -31,7 +31,8 @@ gather_kernel(const T* __restrict__ table, const int32_t* __restrict__ buckets, 
 // ---- gradient of the table ------------------------------------------------------------------------------------------------------
 // A CTA holds several copies of its part of the table in shared memory.  The `lanes` threads of a copy take every copies-th
 // run of AHEAD edges of the CTA's and add their rows to the copy, each thread to columns of its own: no two threads add to one
-// number, so there are no atomics, and the order of the sums depends on the sizes alone.  The copies are summed at the end,
+// number, so there are no atomics, and the order of the sums depends on the sizes, on how g is aligned (its packets) and on the
+// number of multiprocessors.  The copies are summed at the end,
 // the CTAs' sums in a second launch.
 //
 // Large tables leave room for few copies, so few warps, and what counts is how long an addition takes one of them: a run is

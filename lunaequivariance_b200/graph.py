@@ -22,7 +22,11 @@ SOURCE_SEGMENT_EDGES = 32
 # A warp walks a node's edges one after the other, so a node with very many edges would hold one warp for the whole
 # launch.  Rows longer than this are cut into virtual rows of at most this many edges (LunaTPGraph.split_rows).
 ROW_SPLIT_EDGES = 1024
-# Operators that read a row as a whole cut long rows into pieces of this many edges (LunaTPGraph.row_holder).
+# Operators that read a row as a whole cut long rows into pieces of this many edges (LunaTPGraph.row_holder).  Softmax over
+# in-edges, forward / backward in us, pieces of 128, 256 or 512: 1.0 M edges of hubs on 5,003 nodes, FP64, three heads, 62 / 40,
+# 56 / 42, 56 / 44; FP32, eight heads, 42 / 46, 42 / 48, 42 / 50; whole rows 2,460 / 1,240 and 1,090 / 940.  Rows cut where one
+# has more than 512, 1,024 or 2,048: the former 59 / 38, 56 / 42, 75 / 54.  One row of 2,000 among 50,000 of 52, FP64: 114 / 64,
+# whole 156 / 85.
 ROW_PIECE_EDGES = 256
 _TABLE_LIMIT = (1 << 31) - 1024  # entries of a table with 32-bit indices
 

@@ -125,7 +125,9 @@ def graph_softmax(logits, graph, *, mask=None, table=None, buckets=None):
     edges that are ``True``; what stands in the others' logits does not matter, and their result is zero.  A node whose
     edges are all masked, or have logits of minus infinity only, gets zeros.  Where the result is zero nothing flows back.
 
-    The first call with a graph reads its largest degree; make it before a CUDA graph is captured.
+    The first call with a graph reads its largest degree, and makes tables if a node has very many in-edges.  It waits for the
+    GPU; make it before a CUDA graph is captured (``graph.row_holder()`` does that and nothing else).  Traced programs carry the
+    row pointers alone, and walk a node's edges in one warp or one block, however many: graphs with hubs are faster in eager calls.
     """
     if not isinstance(graph, LunaTPGraph):
         raise TypeError("graph must come from make_graph")

@@ -6,7 +6,8 @@ Every block ``mul x l`` of a row is normalised alone: scalars (``0e``) lose thei
 With the irreps of scalars alone, or their number, this is the layer norm of a radial or a readout network.
 
 Float32, float64, bfloat16 and float16 on CUDA, sums in 32 bits (64 for float64); forward, backward and second order (a force
-step differentiates the norm of its radial network twice); the sums of the weights' gradients are reproducible to the bit.
+step differentiates the norm of its radial network twice); the sums of the weights' gradients are the same bits
+for the same sizes, alignment of the tensors and device.
 """
 
 from __future__ import annotations

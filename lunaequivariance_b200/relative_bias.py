@@ -87,7 +87,8 @@ def relative_bias(table, buckets):
     """``table[buckets]`` for a table ``[buckets, heads]`` and int32 ``buckets`` of any shape.
 
     A bucket that is no row of the table (-1 marks an edge without a bias) gives zeros and adds nothing to the table's
-    gradient, which is a sum without atomics: the same bits every time.  Differentiable to any order.
+    gradient, which is a sum without atomics: the same bits for the same sizes, alignment and device.  Sums are held in 32 bits, in 64 for
+    float64.  Differentiable to any order.
     """
     if is_compiling():
         return torch.ops.lunaeq.relative_bias_forward.default(table, buckets)

@@ -332,3 +332,36 @@ def test_sums_by_bucket_behind_a_softmax_of_many_edges(dtype):
     parts = 4 * relative * alpha.reshape(-1, heads) * e.abs().max() + 300 * inner(dtype) * gz.abs()
     allowed = torch.zeros_like(want).index_add_(0, index.long(), parts) + step(dtype) * want.abs()
     assert ((got.double() - want).abs() <= allowed).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_operators_of_the_second_order(dtype):
+    """The operators that a traced program names, with cotangents of either type; third orders are refused in every type."""
+    generator = torch.Generator().manual_seed(2)
+    graph, _ = graph_of([5, 0, 40, 9], generator)
+    z, g, r = (torch.randn(54, 3, generator=generator, dtype=F64).to(dtype).to(DEVICE) for _ in range(3))
+    table = torch.randn(4, 3, generator=generator, dtype=F64).to(dtype).to(DEVICE)
+    buckets = torch.randint(4, (54,), generator=generator, dtype=torch.int32).to(DEVICE)
+    ops = torch.ops.lunaeq
+    alpha, wide = ops.graph_softmax_forward(z, table, buckets, None, graph.dst_rowptr, graph.num_edges)
+    kind = ("test_schema", "test_faketensor")
+    for cotangent in {g.dtype, torch.float32 if dtype in (BF16, F16) else dtype}:
+        args = (alpha, wide, g.to(cotangent), buckets, 4, graph.dst_rowptr, [True, True])
+        torch.library.opcheck(ops.graph_softmax_backward.default, args, test_utils=kind)
+        assert all(t.dtype == dtype for t in ops.graph_softmax_backward(*args))
+        args = (alpha, wide, g.to(cotangent), buckets, r, table, graph.dst_rowptr, [True, True])
+        torch.library.opcheck(ops.graph_softmax_double_backward.default, args, test_utils=kind)
+        halpha, hg = ops.graph_softmax_double_backward(*args)
+        assert halpha.dtype == (F32 if dtype in (BF16, F16) else dtype) and hg.dtype == cotangent
+    # an alpha that was rounded, without what it was before: its own type comes back
+    if dtype in (BF16, F16):
+        leaf = alpha.clone().requires_grad_(True)
+        gz, _ = ops.graph_softmax_backward(leaf, wide[:0], g, buckets, 4, graph.dst_rowptr, [True, False])
+        assert torch.autograd.grad(gz, leaf, r)[0].dtype == dtype
+    for softmax in (lambda z: luna.graph_softmax(z, graph, table=table, buckets=buckets),
+                    lambda z: ops.graph_softmax_forward(z, table, buckets, None, graph.dst_rowptr, graph.num_edges)[0]):
+        leaf = z.clone().requires_grad_(True)
+        first, = torch.autograd.grad(softmax(leaf).square().sum(), leaf, create_graph=True)
+        second, = torch.autograd.grad(first.square().sum(), leaf, create_graph=True)
+        with pytest.raises((NotImplementedError, RuntimeError), match="third-order|does not require grad|autograd"):
+            torch.autograd.grad(second.sum(), leaf)
