@@ -125,6 +125,9 @@ def graph_softmax(logits, graph, *, mask=None, table=None, buckets=None):
     edges that are ``True``; what stands in the others' logits does not matter, and their result is zero.  A node whose
     edges are all masked, or have logits of minus infinity only, gets zeros.  Where the result is zero nothing flows back.
 
+    Of a gradient's gradient, what is asked for with respect to the result itself leaves out a constant of a node's edges, which the
+    softmax takes out behind it; in 16-bit types it reaches the logits from the result before it was rounded, past the result.
+
     The first call with a graph reads its largest degree, and makes tables if a node has very many in-edges.  It waits for the
     GPU; make it before a CUDA graph is captured (``graph.row_holder()`` does that and nothing else).  Traced programs carry the
     row pointers alone, and walk a node's edges in one warp or one block, however many: graphs with hubs are faster in eager calls.
